@@ -22,7 +22,7 @@ OUT = os.path.join(HERE, "hearth-b200-sys", "src", "lib.rs")
 SCALARS = {"int": "c_int", "size_t": "usize", "float": "f32", "double": "f64", "uint8_t": "u8", "int8_t": "i8",
            "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "char": "c_char", "void": "c_void"}
 HANDLES = {"hb200_weight_t": "hb200_weight", "hb200_act_t": "hb200_act", "hb200_batch_t": "hb200_batch",
-           "hb200_gguf_t": "hb200_gguf"}
+           "hb200_gguf_t": "hb200_gguf", "hb200_weight_i8_t": "hb200_weight_i8", "hb200_act_i8_t": "hb200_act_i8"}
 
 
 def strip_comments(text: str) -> str:
@@ -98,7 +98,7 @@ def generate() -> str:
         lines += ["#[repr(C)]", f"pub struct {h} {{", "    _private: [u8; 0],", "}"]
     lines.append("")
     for k, v in constants(text):
-        ty = "usize" if k.startswith(("HB200_NOALLOC", "HB200_MAX", "HB200_PEER")) else "c_int"
+        ty = "usize" if k.startswith(("HB200_NOALLOC", "HB200_MAX", "HB200_PEER", "HB200_I8")) else "c_int"
         lines.append(f"pub const {k}: {ty} = {v};")
     lines += ["", '#[link(name = "hearth_b200")]', 'extern "C" {']
     for name, ret, args in prototypes(text):

@@ -20,6 +20,14 @@ pub struct hb200_batch {
 pub struct hb200_gguf {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct hb200_weight_i8 {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct hb200_act_i8 {
+    _private: [u8; 0],
+}
 
 pub const HB200_OK: c_int = 0;
 pub const HB200_ERR_NOT_INITIALIZED: c_int = -1;
@@ -46,6 +54,8 @@ pub const HB200_PTQ1_0: c_int = 143;
 pub const HB200_MAX_SEQ_LEN: usize = 65535;
 pub const HB200_NOALLOC_MAX_TOKENS: usize = 4;
 pub const HB200_NOALLOC_MAX_COLS: usize = 32768;
+pub const HB200_I8_MAX_COLS: usize = 65536;
+pub const HB200_I8_MAX_ROWS: usize = 8388480;
 pub const HB200_PEER_HANDLE_BYTES: usize = 64;
 pub const HB200_MAX_PEERS: usize = 8;
 
@@ -101,6 +111,25 @@ extern "C" {
     pub fn hb200_dot_rows_dev(w: *mut hb200_weight, a: *mut hb200_act, seq_len: usize, out_dev: *mut f32, ld_out: usize, stream: *mut c_void) -> c_int;
     pub fn hb200_matmul_f32_dev(w: *mut hb200_weight, a: *mut hb200_act, seq_len: usize, out_dev: *mut f32, ld_out: usize, stream: *mut c_void) -> c_int;
     pub fn hb200_matmul_f32_noalloc(w: *mut hb200_weight, x_dev: *const f32, seq_len: usize, out_dev: *mut f32, ld_out: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_weight_i8_upload(n_rows: usize, n_cols: usize, q: *const i8, scales: *const f32, out: *mut *mut hb200_weight_i8) -> c_int;
+    pub fn hb200_weight_i8_upload_rows(n_rows: usize, n_cols: usize, q: *const i8, scales: *const f32, row_begin: usize, row_end: usize, out: *mut *mut hb200_weight_i8) -> c_int;
+    pub fn hb200_weight_i8_upload_dev(n_rows: usize, n_cols: usize, q_dev: *const i8, ld_q: usize, scales_dev: *const f32, stream: *mut c_void, out: *mut *mut hb200_weight_i8) -> c_int;
+    pub fn hb200_weight_i8_quantize_dev(n_rows: usize, n_cols: usize, w_dev: *const f32, ld_w: usize, stream: *mut c_void, out: *mut *mut hb200_weight_i8) -> c_int;
+    pub fn hb200_weight_i8_store_dev(w: *mut hb200_weight_i8, q_dev: *mut i8, ld_q: usize, scales_dev: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn hb200_weight_i8_free(w: *mut hb200_weight_i8) -> c_int;
+    pub fn hb200_weight_i8_info(w: *mut hb200_weight_i8, n_rows: *mut usize, n_cols: *mut usize, resident_bytes: *mut usize, device: *mut c_int) -> c_int;
+    pub fn hb200_act_i8_create(max_seq_len: usize, n_cols: usize, out: *mut *mut hb200_act_i8) -> c_int;
+    pub fn hb200_act_i8_free(a: *mut hb200_act_i8) -> c_int;
+    pub fn hb200_act_i8_info(a: *mut hb200_act_i8, max_seq_len: *mut usize, n_cols: *mut usize, device: *mut c_int) -> c_int;
+    pub fn hb200_act_i8_quantize_dev(a: *mut hb200_act_i8, x_dev: *const f32, ld_x: usize, seq_len: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_act_i8_add_rms_norm_dev(a: *mut hb200_act_i8, x_dev: *const f32, residual_dev: *const f32, ld_x: usize, weight_dev: *const f32, eps: f32, seq_len: usize, sum_dev: *mut f32, ld_sum: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_act_i8_silu_mul_dev(a: *mut hb200_act_i8, gate_dev: *const f32, up_dev: *const f32, ld: usize, seq_len: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_act_i8_load_dev(a: *mut hb200_act_i8, q_dev: *const i8, ld_q: usize, scales_dev: *const f32, seq_len: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_act_i8_store_dev(a: *mut hb200_act_i8, q_dev: *mut i8, ld_q: usize, scales_dev: *mut f32, seq_len: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_act_i8_dequantize_dev(a: *mut hb200_act_i8, out_dev: *mut f32, ld_out: usize, seq_len: usize, stream: *mut c_void) -> c_int;
+    pub fn hb200_matmul_i8_dev(w: *mut hb200_weight_i8, a: *mut hb200_act_i8, seq_len: usize, out_dev: *mut f32, ld_out: usize, accumulate: c_int, stream: *mut c_void) -> c_int;
+    pub fn hb200_matmul_i8(w: *mut hb200_weight_i8, x: *const f32, seq_len: usize, out: *mut f32) -> c_int;
+    pub fn hb200_matmul_i8_kernel(n_rows: usize, n_cols: usize, seq_len: usize) -> *const c_char;
     pub fn hb200_batch_create(out: *mut *mut hb200_batch) -> c_int;
     pub fn hb200_batch_add(b: *mut hb200_batch, w: *mut hb200_weight, a: *mut hb200_act, seq_len: usize, out_dev: *mut f32, ld_out: usize) -> c_int;
     pub fn hb200_batch_seal(b: *mut hb200_batch) -> c_int;

@@ -309,7 +309,7 @@ int check_device_status() {
     if (h != 0) {
         cudaMemset(g_ctx.d_status, 0, sizeof(int));
         // 1..9: mbarrier waits of the tensor-core kernels; 40: bulk copy of x in the eight-token K-quant kernel; 50: carry
-        // of a panel cut between two CTAs (decode matvec); 100 + r: peer rank r's flag
+        // of a panel cut between two CTAs (decode matvec); 60..69: the int8 product; 100 + r: peer rank r's flag
         set_error("a bounded wait inside a kernel expired (code %d); results of that call are invalid", h);
         return HB200_ERR_TIMEOUT;
     }
@@ -359,6 +359,10 @@ int ensure_ctx_act(size_t seq_len, size_t n_cols) {
 namespace hb200 {
 int bound_device() { return g_ctx.ready ? g_ctx.device : -1; }
 int use_slot_of(int slot) { return use_slot(slot); }
+int current_slot() { return g_cur; }
+cudaStream_t slot_stream() { return g_ctx.stream; }
+int slot_sm_count() { return g_ctx.sm_count; }
+int* slot_status() { return g_ctx.d_status; }
 }  // namespace hb200
 
 // Binds slot `slot` to CUDA device `device`: stream, status word, scratch, per-device kernel attributes.
@@ -394,6 +398,7 @@ static int init_slot(int slot, int device) {
     if ((rc = gemm_tc_prepare())) return rc;
     if ((rc = gemm_tcr_prepare())) return rc;
     if ((rc = producers_prepare())) return rc;
+    if ((rc = i8_gemm_prepare(c.sm_count))) return rc;
     if (!g_encode_tiled) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult qres;
@@ -470,6 +475,7 @@ extern "C" int hb200_shutdown(void) {
         for (auto& kv : c.acts) hb200_act_free(kv.second);
         c.acts.clear();
         c.act = nullptr;
+        i8_release_slot(slot);
         if (c.d_in) cudaFree(c.d_in);
         if (c.d_out) cudaFree(c.d_out);
         if (c.d_status) cudaFree(c.d_status);

@@ -93,6 +93,11 @@ void set_error(const char* fmt, ...);
 int bound_device();
 // Makes device slot `slot` (and its CUDA device) current; an error code if that slot is not initialised.
 int use_slot_of(int slot);
+// The current slot, and what a call on it needs: the stream of the host-buffer calls, the SM count, the status word.
+int current_slot();
+cudaStream_t slot_stream();
+int slot_sm_count();
+int* slot_status();
 #define HB_CUDA(expr)                                                                        \
     do {                                                                                     \
         cudaError_t _e = (expr);                                                             \
@@ -324,5 +329,55 @@ int kquant_grid(int kind, int mt, int sm_count, int n_items);
 int launch_kquant_gemv_list(int kind, int mt, const KqMat* mats_dev, const int* chunks_dev, int n_items, int grid, cudaStream_t st,
                             int* status = nullptr);
 int kquant_prepare();
+
+// ---- 8-bit linear path: int8 values with one f32 scale per row (activations: per token, weights: per channel) --------
+// A plane is the int8 matrix in 128-column blocks of rows of 128 bytes, eight rows and 1024 bytes to a group, the 16-byte
+// chunks of a row permuted as the tensor cores' 128-byte swizzle wants them (chunk j of row r at j ^ (r & 7)), so that a
+// contiguous bulk copy of whole groups is a shared-memory operand.  Weights: 128-row tiles, all blocks of a tile in
+// turn (a product streams one contiguous run per tile).  Activations: all row groups of a block in turn (a block's tile
+// of any number of tokens is contiguous).  Columns past n_cols up to the block's end are zero.
+struct I8Plane {
+    int8_t* q;
+    size_t tile_stride;  // bytes between row tiles of (1 << row_shift) rows
+    size_t kb_stride;    // bytes between 128-column blocks
+    int row_shift;       // 7: weights, 3: activations
+};
+enum I8RowOp : int { I8_QUANTIZE = 0, I8_SILU_MUL = 1, I8_ADD_RMS_NORM = 2 };
+constexpr int I8_MAX_COLS = 65536;  // |sum of products| <= 65536 * 128 * 128 = 2^30: exact in int32
+struct I8Rows {
+    const float* x;       // input, gate
+    const float* y;       // residual (may be null), up
+    const float* weight;  // norm weight
+    float* sum;           // norm: x + residual (may be null, may be x or y)
+    size_t ld, ld_sum;    // floats between rows of x and y, of sum
+    int n_cols;
+    float eps;
+    I8Plane plane;
+    float* scales;
+};
+// i8_quant.cu
+int launch_i8_rows(int op, const I8Rows& p, int n_rows, cudaStream_t st);
+int launch_i8_load(const int8_t* q, size_t ld, const float* scales_in, int n_rows, int n_cols, const I8Plane& plane, float* scales, cudaStream_t st);
+int launch_i8_store(const I8Plane& plane, const float* scales, int n_rows, int n_cols, int8_t* q, size_t ld, float* scales_out, cudaStream_t st);
+int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld, cudaStream_t st);
+
+// i8_gemm.cu
+struct I8Product {
+    const int8_t* w;      // weight plane
+    const float* sw;      // scale per weight row
+    const int8_t* a;      // activation plane
+    const float* sx;      // scale per token
+    float* out;           // out[token * ld_out + row]
+    size_t ld_out;
+    size_t a_kb_stride;   // bytes between 128-column blocks of the activation plane
+    int n_rows, n_tok, kb;
+    int accumulate;       // out += result
+    int* status;          // device word for an expired wait
+};
+int i8_gemm_prepare(int sm_count);  // per device: kernel attributes, clusters that fit at once
+int launch_i8_gemm(const I8Product& p, cudaStream_t st);
+const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok);
+// i8_abi.cu: frees what the host-buffer product keeps for a slot.
+void i8_release_slot(int slot);
 
 }  // namespace hb200

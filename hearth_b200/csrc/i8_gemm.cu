@@ -1,0 +1,316 @@
+// Product of the 8-bit linear path: out[s][n] (+)= (sum_k q_w[n][k] q_x[s][k]) * scale_w[n] * scale_x[s], int8 operands
+// with one scale per weight row and one per token, the sum exact in int32.
+//
+// The weight rows are the MMA's M (128 TMEM lanes), the tokens its N (TMEM columns): tcgen05.mma kind::i8, 128 x NTOK x 32.
+// With the channel on the lane a warp's store of one token is 128 contiguous bytes, and a short batch costs no more
+// than its own columns.  Both planes are stored as swizzled shared-memory tiles (common.cuh), so an operand is one
+// contiguous bulk copy: 16 KiB of weights and NTOK * 128 bytes of activations per 128-column block, no tensor map.
+//
+// Few tokens: the time is the weights' way from HBM, and what counts is how many bytes are in flight on how many SMs.
+// A tile of 128 rows is cut along K over the CTAs of a cluster; integer partial sums meet through distributed shared
+// memory (no workspace, no atomics, any order gives the same bits), every CTA finishing its share of the tile.
+// The weight copies of the first stages are issued before the wait on the previous kernel of the stream (programmatic
+// dependent launch): weights are written once, at upload, which synchronises.
+//
+// Every wait on an mbarrier is bounded; on expiry the CTA records a status code, drains its copies, frees its TMEM and
+// returns (its cluster neighbours still meet it at the cluster barriers).
+#include <algorithm>
+
+#include "tc_common.cuh"
+
+namespace hb200 {
+
+namespace {
+
+constexpr int W_TILE = 16384;  // 128 rows x 128 bytes
+constexpr int MAX_SPLIT = 8;   // portable cluster size
+
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Untiled bulk copy: addresses and size are multiples of 16 bytes by the planes' layout.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int4 peer_ld4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// The order of the two multiplications keeps an intermediate of tiny scales out of the subnormals.
+__device__ __forceinline__ float scaled(int acc, float sw, float sx) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), sw), sx); }
+
+template <int NTOK>
+constexpr uint32_t idesc_i8() {  // D = S32, A and B signed int8, both K-major, M = 128, N = NTOK
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NTOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+template <int NTOK>
+struct SplitCfg {
+    static constexpr int X_TILE = NTOK * 128;
+    static constexpr int STAGE = W_TILE + X_TILE;
+    // two CTAs per SM up to 128 tokens
+    static constexpr int STAGES = NTOK <= 32 ? 5 : (NTOK <= 64 ? 4 : (NTOK <= 128 ? 3 : 4));
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
+};
+
+// grid (split, token tiles, row tiles), cluster (split, 1, 1): rank r of a cluster takes blocks [kb * r / split, kb * (r + 1) / split).
+template <int NTOK>
+__global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
+    using C = SplitCfg<NTOK>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ unsigned char dyn[];
+    __shared__ uint64_t full[STAGES], empty[STAGES], done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ float s_sx[NTOK];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = gridDim.x, rank = blockIdx.x;
+    const int tok0 = blockIdx.y * NTOK, row_tile = blockIdx.z, row0 = row_tile * 128;
+    const int n_tok = min(NTOK, p.n_tok - tok0);
+    const int k0 = (int)((long long)p.kb * rank / split), k1 = (int)((long long)p.kb * (rank + 1) / split), nk = k1 - k0;
+    const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t x_bytes = (uint32_t)((n_tok + 7) / 8) * 1024;  // whole groups of eight tokens; other columns of the tile are not stored
+    const int8_t* wp = p.w + ((size_t)row_tile * p.kb + k0) * W_TILE;
+    const int8_t* xp = p.a + (size_t)k0 * p.a_kb_stride + (size_t)tok0 * 128;
+
+    pdl_trigger();
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(&done), 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < nk && i < STAGES; i++) {
+            mbar_expect_tx(smem_u32(&full[i]), W_TILE + x_bytes);
+            bulk_load(ring + i * C::STAGE, wp + (size_t)i * W_TILE, W_TILE, smem_u32(&full[i]));
+        }
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < nk && i < STAGES; i++)
+                bulk_load(ring + i * C::STAGE + W_TILE, xp + (size_t)i * p.a_kb_stride, x_bytes, smem_u32(&full[i]));
+            int issued = min(nk, STAGES);
+            for (int i = STAGES; i < nk; i++) {
+                const int s = i % STAGES;
+                if (!mbar_wait(smem_u32(&empty[s]), (uint32_t)(i / STAGES - 1) & 1u, &abort_flag, p.status, 60)) break;
+                const uint32_t dst = ring + s * C::STAGE;
+                mbar_expect_tx(smem_u32(&full[s]), W_TILE + x_bytes);
+                bulk_load(dst, wp + (size_t)i * W_TILE, W_TILE, smem_u32(&full[s]));
+                bulk_load(dst + W_TILE, xp + (size_t)i * p.a_kb_stride, x_bytes, smem_u32(&full[s]));
+                issued = i + 1;
+            }
+            if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
+                for (int i = max(0, issued - STAGES); i < issued; i++)
+                    for (uint32_t t = 0; t < SPIN_LIMIT && !mbar_try(smem_u32(&full[i % STAGES]), (uint32_t)(i / STAGES) & 1u); t++) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int i = 0; i < nk && ok; i++) {
+                const int s = i % STAGES;
+                ok = mbar_wait(smem_u32(&full[s]), (uint32_t)(i / STAGES) & 1u, &abort_flag, p.status, 61);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t ad = make_desc(ring + s * C::STAGE), bd = make_desc(ring + s * C::STAGE + W_TILE);
+#pragma unroll
+                for (int j = 0; j < 4; j++) mma_i8(tmem, ad + 2 * j, bd + 2 * j, idesc_i8<NTOK>(), (i | j) != 0);
+                tc_commit(smem_u32(&empty[s]));
+            }
+            tc_commit(smem_u32(&done));
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        for (int t = lane; t < NTOK; t += 32) s_sx[t] = t < n_tok ? p.sx[tok0 + t] : 0.f;
+    }
+    const bool ok = mbar_wait(smem_u32(&done), 0, &abort_flag, p.status, 62);
+    __syncthreads();
+    tc_fence_after();
+
+    const int row = row0 + warp * 32 + lane;
+    const uint32_t tm = tmem + ((uint32_t)(warp * 32) << 16);
+    if (split == 1) {
+        const float sw = row < p.n_rows ? p.sw[row] : 0.f;
+        float* out = p.out + (size_t)tok0 * p.ld_out + row;
+        for (int c0 = 0; c0 < n_tok; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(tm + c0, v);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (ok && row < p.n_rows && c0 + j < n_tok) {
+                    float* o = out + (size_t)(c0 + j) * p.ld_out;
+                    const float r = scaled((int)v[j], sw, s_sx[c0 + j]);
+                    *o = p.accumulate ? __fadd_rn(*o, r) : r;
+                }
+        }
+    } else {
+        // partial sums of the tile, [token][128 rows], in the memory of the ring: every copy has landed and been read
+        int* part = reinterpret_cast<int*>(dyn + (ring - smem_u32(dyn)));
+        for (int c0 = 0; c0 < n_tok; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(tm + c0, v);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (c0 + j < n_tok) part[(c0 + j) * 128 + warp * 32 + lane] = (int)v[j];
+        }
+        cluster_sync();
+        const int n_vec = n_tok * 32;
+        const int v0 = n_vec * rank / split, v1 = n_vec * (rank + 1) / split;
+        const bool vec = (p.ld_out % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0);
+        for (int i = v0 + tid; i < v1; i += 128) {
+            int4 s = make_int4(0, 0, 0, 0);
+            for (int r = 0; r < split; r++) {
+                const int4 t = peer_ld4(peer_smem(ring + i * 16, r));
+                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+            }
+            const int tok = i >> 5, r4 = row0 + (i & 31) * 4;
+            const float sx = s_sx[tok];
+            float* o = p.out + (size_t)(tok0 + tok) * p.ld_out + r4;
+            if (!ok) continue;
+            if (vec && r4 + 3 < p.n_rows) {
+                const float4 w = *reinterpret_cast<const float4*>(p.sw + r4);
+                float4 f = make_float4(scaled(s.x, w.x, sx), scaled(s.y, w.y, sx), scaled(s.z, w.z, sx), scaled(s.w, w.w, sx));
+                if (p.accumulate) {
+                    const float4 b = *reinterpret_cast<const float4*>(o);
+                    f = make_float4(__fadd_rn(b.x, f.x), __fadd_rn(b.y, f.y), __fadd_rn(b.z, f.z), __fadd_rn(b.w, f.w));
+                }
+                *reinterpret_cast<float4*>(o) = f;
+            } else {
+                const int q[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (r4 + j < p.n_rows) {
+                        const float f = scaled(q[j], p.sw[r4 + j], sx);
+                        o[j] = p.accumulate ? __fadd_rn(o[j], f) : f;
+                    }
+            }
+        }
+        cluster_sync();  // a neighbour may still be reading this CTA's partial sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+    }
+}
+
+struct Plan {
+    int ntok, split;
+};
+
+int g_sm_count = 148;
+
+int ntok_of(int n_tok) { return n_tok <= 16 ? 16 : n_tok <= 32 ? 32 : n_tok <= 64 ? 64 : n_tok <= 128 ? 128 : 256; }
+
+Plan plan(int n_rows, int kb, int n_tok) {
+    Plan best = {ntok_of(n_tok), 1};
+    const long long tiles = (long long)((n_rows + 127) / 128) * ((n_tok + best.ntok - 1) / best.ntok);
+    const int slots = g_sm_count * (best.ntok <= 128 ? 2 : 1);
+    double best_t = 1e30;
+    for (int s = 1; s <= MAX_SPLIT && s <= kb; s++) {
+        const long long waves = (tiles * s + slots - 1) / slots;
+        const double t = waves * ((kb + s - 1) / s + 2.0 + (s > 1 ? 1.0 : 0.0));
+        if (t < best_t) { best_t = t; best.split = s; }
+    }
+    return best;
+}
+
+template <int NTOK>
+int launch_split(const I8Product& p, int split, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, (p.n_tok + NTOK - 1) / NTOK, (p.n_rows + 127) / 128);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = SplitCfg<NTOK>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    HB_CUDA(cudaLaunchKernelEx(&cfg, i8_split_kernel<NTOK>, p));
+    return 0;
+}
+
+}  // namespace
+
+int i8_gemm_prepare(int sm_count) {
+    g_sm_count = sm_count;
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<16>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<32>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<64>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<128>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<256>::SMEM));
+    return 0;
+}
+
+int launch_i8_gemm(const I8Product& p, cudaStream_t st) {
+    const Plan pl = plan(p.n_rows, p.kb, p.n_tok);
+    switch (pl.ntok) {
+        case 16: return launch_split<16>(p, pl.split, st);
+        case 32: return launch_split<32>(p, pl.split, st);
+        case 64: return launch_split<64>(p, pl.split, st);
+        case 128: return launch_split<128>(p, pl.split, st);
+        default: return launch_split<256>(p, pl.split, st);
+    }
+}
+
+const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok) {
+    const Plan pl = plan(n_rows, kb, n_tok);
+    switch (pl.ntok) {
+        case 16: return pl.split > 1 ? "i8_tcgen05_n16_split" : "i8_tcgen05_n16";
+        case 32: return pl.split > 1 ? "i8_tcgen05_n32_split" : "i8_tcgen05_n32";
+        case 64: return pl.split > 1 ? "i8_tcgen05_n64_split" : "i8_tcgen05_n64";
+        case 128: return pl.split > 1 ? "i8_tcgen05_n128_split" : "i8_tcgen05_n128";
+        default: return pl.split > 1 ? "i8_tcgen05_n256_split" : "i8_tcgen05_n256";
+    }
+}
+
+}  // namespace hb200

@@ -1,0 +1,318 @@
+// Rows of the 8-bit linear path: f32 rows -> int8 values with ONE f32 scale per row, in the tiled plane the product
+// kernels (i8_gemm.cu) read, plus the moves between that plane and row-major tensors.
+//
+//   quantize       v = x
+//   silu_mul       v = g / (1 + exp(-g)) * u
+//   add_rms_norm   h = x + r (written out), v = weight * h, and the row's factor f = 1 / sqrt(mean(h^2) + eps)
+//   then           a = max |v|,  q = rint(v * (127 / a)),  scale = a / 127 (* f)
+//
+// The norm's factor multiplies every value of its row, so it cancels out of q and only the scale carries it: one pass
+// over the row computes h, the maximum and the sum of squares together, and the int8 values do not depend on the order
+// of that sum.  All steps are f32 with IEEE rounding (h, v, 127 / a and the product each rounded once), so q is
+// determined to the last bit; never compile this file with fast-math.  A row whose maximum is below I8_MIN_MAX (2^-100,
+// where 127 / a would leave the range of f32) is stored as zeros with scale 0.  A row with an infinity or a NaN in it (or
+// whose sum of squares overflows) is stored as zeros with scale NaN, so whatever is computed from it is NaN, too.
+//
+// HBM-bound: 4 B (quantize, + 4 silu_mul, + 8 add_rms_norm) read or written per element and 1 B written.  One CTA per
+// row keeps the row in registers between the reduction and the rounding (up to 32 values a thread); longer rows are
+// read twice.
+//
+// Reference counterparts with a scale per 32 columns: ops::rms_norm_q8 and ops::silu_mul_q8
+// (hearth-llm/src/ops.rs:273-306, :442-504), quantize_q8_0 (hearth-quant/src/q8_0.rs:20-51).
+#include "common.cuh"
+
+namespace hb200 {
+
+namespace {
+
+constexpr float I8_MIN_MAX = 7.888609052210118e-31f;  // 2^-100
+
+// Programmatic dependent launch: the next kernel of the stream may start its prologue now; this one touches nothing a
+// predecessor wrote (or reads) before the wait.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// 16-byte chunk of (row, column): column c's byte is at chunk_addr + (c & 15).
+__device__ __forceinline__ size_t plane_off(const I8Plane& p, int row, int c) {
+    const size_t tile = (size_t)(row >> p.row_shift) * p.tile_stride + (size_t)(c >> 7) * p.kb_stride;
+    const int r = row & ((1 << p.row_shift) - 1);
+    return tile + (size_t)r * 128 + (size_t)((((c >> 4) & 7) ^ (r & 7)) << 4) + (c & 15);
+}
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    const uint32_t lo = __byte_perm((uint32_t)a, (uint32_t)b, 0x0040);
+    const uint32_t hi = __byte_perm((uint32_t)c, (uint32_t)d, 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+
+template <bool VEC>
+__device__ __forceinline__ float4 read4(const float* row, int c, int n) {
+    if (VEC) return c < n ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v;
+    v.x = c < n ? row[c] : 0.f;
+    v.y = c + 1 < n ? row[c + 1] : 0.f;
+    v.z = c + 2 < n ? row[c + 2] : 0.f;
+    v.w = c + 3 < n ? row[c + 3] : 0.f;
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void write4(float* row, int c, int n, float4 v) {
+    if (VEC) {
+        if (c < n) *reinterpret_cast<float4*>(row + c) = v;
+        return;
+    }
+    if (c < n) row[c] = v.x;
+    if (c + 1 < n) row[c + 1] = v.y;
+    if (c + 2 < n) row[c + 2] = v.z;
+    if (c + 3 < n) row[c + 3] = v.w;
+}
+
+__device__ __forceinline__ float silu_mul1(float g, float u) { return __fmul_rn(__fdiv_rn(g, __fadd_rn(1.0f, expf(-g))), u); }
+
+// The four values v of columns c .. c + 3 (zero past the end); the norm adds h * h to `sq` and writes h.
+template <int OP, bool VEC>
+__device__ __forceinline__ float4 value4(const I8Rows& p, size_t row, int c, float& sq) {
+    const float4 x = read4<VEC>(p.x + row * p.ld, c, p.n_cols);
+    if (OP == I8_QUANTIZE) return x;
+    if (OP == I8_SILU_MUL) {
+        const float4 u = read4<VEC>(p.y + row * p.ld, c, p.n_cols);
+        return make_float4(silu_mul1(x.x, u.x), silu_mul1(x.y, u.y), silu_mul1(x.z, u.z), silu_mul1(x.w, u.w));
+    }
+    float4 h = x;
+    if (p.y) {
+        const float4 r = read4<VEC>(p.y + row * p.ld, c, p.n_cols);
+        h = make_float4(__fadd_rn(x.x, r.x), __fadd_rn(x.y, r.y), __fadd_rn(x.z, r.z), __fadd_rn(x.w, r.w));
+    }
+    if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols, h);
+    sq = fmaf(h.x, h.x, sq);
+    sq = fmaf(h.y, h.y, sq);
+    sq = fmaf(h.z, h.z, sq);
+    sq = fmaf(h.w, h.w, sq);
+    const float4 w = read4<VEC>(p.weight, c, p.n_cols);
+    return make_float4(__fmul_rn(w.x, h.x), __fmul_rn(w.y, h.y), __fmul_rn(w.z, h.z), __fmul_rn(w.w, h.w));
+}
+
+// The same values a second time, for rows that do not fit the registers: the norm reads h back where it was written
+// (x or r may be the same memory as the sum).
+template <int OP, bool VEC>
+__device__ __forceinline__ float4 value4_again(const I8Rows& p, size_t row, int c) {
+    if (OP == I8_ADD_RMS_NORM && p.sum) {
+        const float4 h = read4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols);
+        const float4 w = read4<VEC>(p.weight, c, p.n_cols);
+        return make_float4(__fmul_rn(w.x, h.x), __fmul_rn(w.y, h.y), __fmul_rn(w.z, h.z), __fmul_rn(w.w, h.w));
+    }
+    float unused = 0.f;
+    return value4<OP, VEC>(p, row, c, unused);
+}
+
+__device__ __forceinline__ uint32_t absmax4(uint32_t m, float4 v) {
+    // as integers the bits of |v| order like the numbers, and a NaN is above infinity: nothing gets lost
+    m = max(m, __float_as_uint(v.x) & 0x7FFFFFFFu);
+    m = max(m, __float_as_uint(v.y) & 0x7FFFFFFFu);
+    m = max(m, __float_as_uint(v.z) & 0x7FFFFFFFu);
+    return max(m, __float_as_uint(v.w) & 0x7FFFFFFFu);
+}
+
+__device__ __forceinline__ uint32_t round4(float4 v, float inv) {
+    return pack4(__float2int_rn(__fmul_rn(v.x, inv)), __float2int_rn(__fmul_rn(v.y, inv)), __float2int_rn(__fmul_rn(v.z, inv)),
+                 __float2int_rn(__fmul_rn(v.w, inv)));
+}
+
+// One CTA per row.  NV = float4s of the row a thread keeps (0: the row is read twice).
+template <int OP, int NV, bool VEC>
+__global__ void __launch_bounds__(1024) i8_rows_kernel(const I8Rows p) {
+    __shared__ uint32_t s_max[32];
+    __shared__ float s_sq[32];
+    const int row = blockIdx.x;
+    const int step = blockDim.x * 4;
+    pdl_trigger();
+    pdl_wait();
+    float4 v[NV > 0 ? NV : 1];
+    uint32_t m = 0;
+    float sq = 0.f;
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            v[i] = value4<OP, VEC>(p, row, threadIdx.x * 4 + i * step, sq);
+            m = absmax4(m, v[i]);
+        }
+    } else {
+        for (int c = threadIdx.x * 4; c < p.n_cols; c += step) m = absmax4(m, value4<OP, VEC>(p, row, c, sq));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (OP == I8_ADD_RMS_NORM) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    }
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps > 1) {
+        if (lane == 0) {
+            s_max[threadIdx.x >> 5] = m;
+            if (OP == I8_ADD_RMS_NORM) s_sq[threadIdx.x >> 5] = sq;
+        }
+        __syncthreads();
+        m = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[lane] : 0u);
+        if (OP == I8_ADD_RMS_NORM) {
+            sq = lane < warps ? s_sq[lane] : 0.f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        }
+    }
+    const float a = __uint_as_float(m);
+    const bool bad = m >= 0x7F800000u || (OP == I8_ADD_RMS_NORM && !(sq <= 3.4028234e38f));
+    const float inv = (!bad && a >= I8_MIN_MAX) ? __fdiv_rn(127.0f, a) : 0.0f;
+    if (threadIdx.x == 0) {
+        float scale = (a >= I8_MIN_MAX) ? __fdiv_rn(a, 127.0f) : 0.0f;
+        if (OP == I8_ADD_RMS_NORM) scale = __fmul_rn(scale, __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sq, (float)p.n_cols), p.eps))));
+        p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : scale;
+    }
+    const int padded = (p.n_cols + 127) & ~127;
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = threadIdx.x * 4 + i * step;
+            if (c < padded) *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(v[i], inv);
+        }
+    } else {
+        for (int c = threadIdx.x * 4; c < padded; c += step)
+            *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(value4_again<OP, VEC>(p, row, c), inv);
+    }
+}
+
+// Row-major int8 rows (`ld` bytes apart) -> plane; columns past n_cols become zero.  grid (columns / 512, rows).
+__global__ void __launch_bounds__(128) i8_load_kernel(const int8_t* q, size_t ld, const float* scales_in, int n_rows, int n_cols, I8Plane plane,
+                                                      float* scales) {
+    pdl_trigger();
+    pdl_wait();
+    const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
+    const int padded = (n_cols + 127) & ~127;
+    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
+        if (c < padded) {
+            const int8_t* src = q + (size_t)row * ld;
+            uint32_t v = 0;
+            if (c + 3 < n_cols && ((reinterpret_cast<uintptr_t>(src + c) & 3) == 0)) {
+                v = *reinterpret_cast<const uint32_t*>(src + c);
+            } else {
+                for (int i = 0; i < 4; i++)
+                    if (c + i < n_cols) v |= (uint32_t)(uint8_t)src[c + i] << (8 * i);
+            }
+            *reinterpret_cast<uint32_t*>(plane.q + plane_off(plane, row, c)) = v;
+        }
+        if (c == 0) scales[row] = scales_in[row];
+    }
+}
+
+// Plane -> row-major int8 rows and / or scales.
+__global__ void __launch_bounds__(128) i8_store_kernel(I8Plane plane, const float* scales, int n_rows, int n_cols, int8_t* q, size_t ld,
+                                                       float* scales_out) {
+    pdl_trigger();
+    pdl_wait();
+    const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
+    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
+        if (q && c < n_cols) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(plane.q + plane_off(plane, row, c));
+            int8_t* dst = q + (size_t)row * ld + c;
+            if (c + 3 < n_cols && ((reinterpret_cast<uintptr_t>(dst) & 3) == 0)) {
+                *reinterpret_cast<uint32_t*>(dst) = v;
+            } else {
+                for (int i = 0; i < 4; i++)
+                    if (c + i < n_cols) dst[i] = (int8_t)(v >> (8 * i));
+            }
+        }
+        if (scales_out && c == 0) scales_out[row] = scales[row];
+    }
+}
+
+// Plane -> the f32 values it stands for, q * scale.
+template <bool VEC>
+__global__ void __launch_bounds__(128) i8_dequantize_kernel(I8Plane plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld) {
+    pdl_trigger();
+    pdl_wait();
+    const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
+    if (c >= n_cols) return;
+    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(plane.q + plane_off(plane, row, c));
+        const float s = scales[row];
+        const float4 f = make_float4(__fmul_rn((float)(int8_t)(v), s), __fmul_rn((float)(int8_t)(v >> 8), s),
+                                     __fmul_rn((float)(int8_t)(v >> 16), s), __fmul_rn((float)(int8_t)(v >> 24), s));
+        write4<VEC>(out + (size_t)row * ld, c, n_cols, f);
+    }
+}
+
+bool vec_rows(const void* p, size_t ld) { return ((reinterpret_cast<uintptr_t>(p) & 15) == 0) && (ld % 4 == 0); }
+
+template <int OP, int NV>
+int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_rows);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA(vec ? cudaLaunchKernelEx(&cfg, i8_rows_kernel<OP, NV, true>, p) : cudaLaunchKernelEx(&cfg, i8_rows_kernel<OP, NV, false>, p));
+    return 0;
+}
+
+template <int OP>
+int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
+    const int quads = ((p.n_cols + 127) & ~127) / 4;  // float4s of a padded row
+    // Few rows: as many threads per row as there are float4s (latency).  Many rows: four float4s a thread, so that the
+    // loads of a row are in flight together and several rows share an SM.
+    const int want = n_rows >= 256 ? 4 : 1;
+    int nv = want;
+    while ((quads + nv - 1) / nv > 1024) nv *= 2;
+    if (nv > 8) return launch_rows_nv<OP, 0>(p, n_rows, 1024, vec, st);
+    const int threads = ((quads + nv - 1) / nv + 31) / 32 * 32;
+    switch (nv) {
+        case 1: return launch_rows_nv<OP, 1>(p, n_rows, threads, vec, st);
+        case 2: return launch_rows_nv<OP, 2>(p, n_rows, threads, vec, st);
+        case 4: return launch_rows_nv<OP, 4>(p, n_rows, threads, vec, st);
+        default: return launch_rows_nv<OP, 8>(p, n_rows, threads, vec, st);
+    }
+}
+
+dim3 move_grid(int n_rows, int n_cols) { return dim3((((n_cols + 127) & ~127) + 511) / 512, n_rows < 65535 ? n_rows : 65535); }
+
+}  // namespace
+
+int launch_i8_rows(int op, const I8Rows& p, int n_rows, cudaStream_t st) {
+    if (n_rows <= 0) return 0;
+    bool vec = (p.n_cols % 4 == 0) && vec_rows(p.x, p.ld);
+    if (p.y) vec = vec && vec_rows(p.y, p.ld);
+    if (p.weight) vec = vec && vec_rows(p.weight, 0);
+    if (p.sum) vec = vec && vec_rows(p.sum, p.ld_sum);
+    switch (op) {
+        case I8_QUANTIZE: return launch_rows_op<I8_QUANTIZE>(p, n_rows, vec, st);
+        case I8_SILU_MUL: return launch_rows_op<I8_SILU_MUL>(p, n_rows, vec, st);
+        default: return launch_rows_op<I8_ADD_RMS_NORM>(p, n_rows, vec, st);
+    }
+}
+
+int launch_i8_load(const int8_t* q, size_t ld, const float* scales_in, int n_rows, int n_cols, const I8Plane& plane, float* scales, cudaStream_t st) {
+    if (n_rows <= 0) return 0;
+    i8_load_kernel<<<move_grid(n_rows, n_cols), 128, 0, st>>>(q, ld, scales_in, n_rows, n_cols, plane, scales);
+    HB_CUDA(cudaGetLastError());
+    return 0;
+}
+
+int launch_i8_store(const I8Plane& plane, const float* scales, int n_rows, int n_cols, int8_t* q, size_t ld, float* scales_out, cudaStream_t st) {
+    if (n_rows <= 0) return 0;
+    i8_store_kernel<<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, q, ld, scales_out);
+    HB_CUDA(cudaGetLastError());
+    return 0;
+}
+
+int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld, cudaStream_t st) {
+    if (n_rows <= 0) return 0;
+    if ((n_cols % 4 == 0) && vec_rows(out, ld))
+        i8_dequantize_kernel<true><<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, out, ld);
+    else
+        i8_dequantize_kernel<false><<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, out, ld);
+    HB_CUDA(cudaGetLastError());
+    return 0;
+}
+
+}  // namespace hb200

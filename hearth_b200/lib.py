@@ -94,6 +94,25 @@ SIGNATURES = {
     "hb200_dot_rows_dev": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
     "hb200_matmul_f32_dev": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
     "hb200_matmul_f32_noalloc": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
+    "hb200_weight_i8_upload": (_int, [_sz, _sz, _vp, _vp, C.POINTER(_vp)]),
+    "hb200_weight_i8_upload_rows": (_int, [_sz, _sz, _vp, _vp, _sz, _sz, C.POINTER(_vp)]),
+    "hb200_weight_i8_upload_dev": (_int, [_sz, _sz, _vp, _sz, _vp, _vp, C.POINTER(_vp)]),
+    "hb200_weight_i8_quantize_dev": (_int, [_sz, _sz, _vp, _sz, _vp, C.POINTER(_vp)]),
+    "hb200_weight_i8_store_dev": (_int, [_vp, _vp, _sz, _vp, _vp]),
+    "hb200_weight_i8_free": (_int, [_vp]),
+    "hb200_weight_i8_info": (_int, [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_int)]),
+    "hb200_act_i8_create": (_int, [_sz, _sz, C.POINTER(_vp)]),
+    "hb200_act_i8_free": (_int, [_vp]),
+    "hb200_act_i8_info": (_int, [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_int)]),
+    "hb200_act_i8_quantize_dev": (_int, [_vp, _vp, _sz, _sz, _vp]),
+    "hb200_act_i8_add_rms_norm_dev": (_int, [_vp, _vp, _vp, _sz, _vp, C.c_float, _sz, _vp, _sz, _vp]),
+    "hb200_act_i8_silu_mul_dev": (_int, [_vp, _vp, _vp, _sz, _sz, _vp]),
+    "hb200_act_i8_load_dev": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
+    "hb200_act_i8_store_dev": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
+    "hb200_act_i8_dequantize_dev": (_int, [_vp, _vp, _sz, _sz, _vp]),
+    "hb200_matmul_i8_dev": (_int, [_vp, _vp, _sz, _vp, _sz, _int, _vp]),
+    "hb200_matmul_i8": (_int, [_vp, _vp, _sz, _vp]),
+    "hb200_matmul_i8_kernel": (C.c_char_p, [_sz, _sz, _sz]),
     "hb200_batch_create": (_int, [C.POINTER(_vp)]),
     "hb200_batch_add": (_int, [_vp, _vp, _vp, _sz, _vp, _sz]),
     "hb200_batch_seal": (_int, [_vp]),

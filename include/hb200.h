@@ -76,6 +76,8 @@ typedef struct hb200_weight *hb200_weight_t; /* resident weight matrix */
 typedef struct hb200_act *hb200_act_t;       /* resident activation (f32 and Q8_0 forms) */
 typedef struct hb200_batch *hb200_batch_t;   /* recorded list of dot-row ops, one launch */
 typedef struct hb200_gguf *hb200_gguf_t;     /* a mapped GGUF model file */
+typedef struct hb200_weight_i8 *hb200_weight_i8_t; /* resident int8 weight matrix with a scale per row */
+typedef struct hb200_act_i8 *hb200_act_i8_t;       /* resident int8 activation with a scale per token */
 
 /* ---- lifecycle ---------------------------------------------------------- */
 
@@ -360,6 +362,86 @@ HB200_API int hb200_matmul_f32_dev(hb200_weight_t w, hb200_act_t a, size_t seq_l
 #define HB200_NOALLOC_MAX_COLS 32768
 HB200_API int hb200_matmul_f32_noalloc(hb200_weight_t w, const float *x_dev, size_t seq_len, float *out_dev,
                                        size_t ld_out, void *stream);
+
+/* ---- 8-bit linear path: one scale per token, one per weight row ------------ */
+
+/* The block formats above carry a scale for every 32 or 128 columns, so their integer sums end after 32 columns.  This
+ * path is for weights that have ONE f32 scale per row (output channel) and activations that have one per token: the
+ * whole sum over the columns is an integer, exact in int32, and the tensor cores run through it:
+ *
+ *   out[s][n] = (sum_k q_w[n][k] * q_x[s][k]) * scale_w[n] * scale_x[s]        (f32, multiplied in this order)
+ *
+ * No counterpart in the reference; the calls stand beside its quantizer, fused producers and matmul
+ * (hearth-quant/src/q8_0.rs:20-51, hearth-llm/src/ops.rs:273-306, :442-504, hearth-llm/src/model/matmul.rs:580-674).
+ *
+ * Rounding a row v to 8 bits: a = max |v|, q = v * (127 / a) rounded to the nearest integer (ties to even), scale = a /
+ * 127; every step is one f32 operation rounded to nearest, so the integers are determined to the last one.  A row with
+ * a < 2^-100 becomes zeros with scale 0.  A row holding an infinity or a NaN becomes zeros with scale NaN: every output
+ * of that token is NaN, and no other token's.  Values handed in by the caller may use all of -128 .. 127.
+ *
+ * Limits: n_cols <= HB200_I8_MAX_COLS, n_rows <= HB200_I8_MAX_ROWS, HB200_MAX_SEQ_LEN tokens; beyond them
+ * HB200_ERR_TOO_LARGE.  Rows of f32 inputs and outputs are `ld` floats apart (ld >= the row's length, any alignment;
+ * multiples of four and 16-byte-aligned bases are faster).  _dev calls enqueue on `stream` (of the handle's device) and
+ * return; they keep no scratch, so calls on different handles may overlap and several products may read one activation
+ * at once.  A call that writes an activation must be ordered behind the calls that read it, like any buffer.  seq_len 0
+ * is a no-op.  Rows of an activation or an output behind seq_len, and output columns behind n_rows, are left as they
+ * were. */
+#define HB200_I8_MAX_COLS 65536
+#define HB200_I8_MAX_ROWS 8388480
+/* int8 values [n_rows][n_cols] and n_rows scales, host memory; the copy on the device is re-tiled. */
+HB200_API int hb200_weight_i8_upload(size_t n_rows, size_t n_cols, const int8_t *q, const float *scales,
+                                     hb200_weight_i8_t *out);
+/* Rows [row_begin, row_end) only (see hb200_weight_upload_rows). */
+HB200_API int hb200_weight_i8_upload_rows(size_t n_rows, size_t n_cols, const int8_t *q, const float *scales,
+                                          size_t row_begin, size_t row_end, hb200_weight_i8_t *out);
+/* The same from device memory, rows ld_q bytes apart, read on `stream`.  This call and the next synchronise `stream`
+ * (the weight is complete when they return), so they cannot be captured into a graph. */
+HB200_API int hb200_weight_i8_upload_dev(size_t n_rows, size_t n_cols, const int8_t *q_dev, size_t ld_q,
+                                         const float *scales_dev, void *stream, hb200_weight_i8_t *out);
+/* Rounds f32 weights [n_rows][n_cols], rows ld_w floats apart in device memory, to 8 bits row by row. */
+HB200_API int hb200_weight_i8_quantize_dev(size_t n_rows, size_t n_cols, const float *w_dev, size_t ld_w, void *stream,
+                                           hb200_weight_i8_t *out);
+/* Row-major values (rows ld_q bytes apart) and scales of a weight; either pointer may be null. */
+HB200_API int hb200_weight_i8_store_dev(hb200_weight_i8_t w, int8_t *q_dev, size_t ld_q, float *scales_dev,
+                                        void *stream);
+HB200_API int hb200_weight_i8_free(hb200_weight_i8_t w);
+/* Shape, resident bytes and CUDA device; any output may be null. */
+HB200_API int hb200_weight_i8_info(hb200_weight_i8_t w, size_t *n_rows, size_t *n_cols, size_t *resident_bytes,
+                                   int *device);
+
+/* Room for max_seq_len tokens of n_cols int8 values and a scale each. */
+HB200_API int hb200_act_i8_create(size_t max_seq_len, size_t n_cols, hb200_act_i8_t *out);
+HB200_API int hb200_act_i8_free(hb200_act_i8_t a);
+HB200_API int hb200_act_i8_info(hb200_act_i8_t a, size_t *max_seq_len, size_t *n_cols, int *device);
+/* Rounds f32 rows [seq_len][n_cols] to 8 bits. */
+HB200_API int hb200_act_i8_quantize_dev(hb200_act_i8_t a, const float *x_dev, size_t ld_x, size_t seq_len, void *stream);
+/* The residual's addition and the norm in front of a projection: h = x + residual (residual_dev may be null: h = x; its
+ * rows are ld_x apart, too), written to sum_dev unless that is null (sum_dev may be x_dev or residual_dev, then with
+ * ld_sum = ld_x); then v = weight * h is rounded to 8 bits and its scale multiplied by 1 / sqrt(mean(h^2) + eps).
+ * The integers therefore do not depend on how the mean is summed.  eps > 0.  h^2 has to stay in the range of f32. */
+HB200_API int hb200_act_i8_add_rms_norm_dev(hb200_act_i8_t a, const float *x_dev, const float *residual_dev, size_t ld_x,
+                                            const float *weight_dev, float eps, size_t seq_len, float *sum_dev,
+                                            size_t ld_sum, void *stream);
+/* gate / (1 + exp(-gate)) * up, rounded to 8 bits; rows of both are ld floats apart (ld = 2 * n_cols for the halves of
+ * one buffer that a product of gate and up together wrote). */
+HB200_API int hb200_act_i8_silu_mul_dev(hb200_act_i8_t a, const float *gate_dev, const float *up_dev, size_t ld,
+                                        size_t seq_len, void *stream);
+/* Caller-made values (rows ld_q bytes apart) and scales into `a`, and back out (either pointer may be null). */
+HB200_API int hb200_act_i8_load_dev(hb200_act_i8_t a, const int8_t *q_dev, size_t ld_q, const float *scales_dev,
+                                    size_t seq_len, void *stream);
+HB200_API int hb200_act_i8_store_dev(hb200_act_i8_t a, int8_t *q_dev, size_t ld_q, float *scales_dev, size_t seq_len,
+                                     void *stream);
+/* The f32 values q * scale of the first seq_len tokens. */
+HB200_API int hb200_act_i8_dequantize_dev(hb200_act_i8_t a, float *out_dev, size_t ld_out, size_t seq_len, void *stream);
+
+/* out[s * ld_out + n] = result, or += result (one f32 addition) with accumulate != 0: the residual's addition of an
+ * output projection. */
+HB200_API int hb200_matmul_i8_dev(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, float *out_dev, size_t ld_out,
+                                  int accumulate, void *stream);
+/* Host buffers: x f32 [seq_len][n_cols] is uploaded and rounded to 8 bits, out f32 [seq_len][n_rows]. */
+HB200_API int hb200_matmul_i8(hb200_weight_i8_t w, const float *x, size_t seq_len, float *out);
+/* Name of the kernel variant that serves a product of this shape ("none" outside the limits); needs no device. */
+HB200_API const char *hb200_matmul_i8_kernel(size_t n_rows, size_t n_cols, size_t seq_len);
 
 /* ---- recorded batches --------------------------------------------------- */
 
