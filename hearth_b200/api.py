@@ -455,44 +455,53 @@ def matmul_f32_noalloc(w: Weight, x_dev, out_dev, ld_out: int | None = None, str
 
 # ---- 8-bit linear path: one scale per token, one per weight row -----------------------------------
 
+_F32 = _I8 = _raw_stream = None  # torch.float32, torch.int8 and the current stream's address of a device
+
+
+def _i8_torch() -> None:
+    """Binds the torch names the calls below use: at one token a call's checks would otherwise cost more than its kernel."""
+    global _F32, _I8, _raw_stream
+    import torch
+    _F32, _I8 = torch.float32, torch.int8
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _i8_rows(name: str, t, dtype, n_cols: int, rows: int, device: int):
     """Address and row stride (elements) of a CUDA tensor of at least `rows` rows of n_cols values, or a refusal."""
     if t is None:
         raise Hb200Error(-5, f"{name}: null tensor")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise Hb200Error(-4, f"{name}: on {t.device}, the handle lives on cuda:{device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise Hb200Error(-4, f"{name}: {t.dtype} where {dtype} is wanted")
-    if t.dim() == 1 and rows <= 1:
-        t = t.unsqueeze(0)
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < n_cols or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise Hb200Error(-4, f"{name}: shape {tuple(t.shape)}, strides {t.stride()} where {rows} rows of {n_cols} adjacent values are wanted")
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), n_cols)
-    return C.c_void_p(t.data_ptr()), ld
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 1 and rows <= 1:
+        shape, stride = (1, shape[0]), (shape[0], stride[0])
+    if len(shape) != 2 or shape[0] < rows or shape[1] < n_cols or (stride[1] != 1 and shape[1] > 1):
+        raise Hb200Error(-4, f"{name}: shape {tuple(shape)}, strides {stride} where {rows} rows of {n_cols} adjacent values are wanted")
+    return t.data_ptr(), stride[0] if shape[0] > 1 or stride[0] > n_cols else n_cols
 
 
 def _i8_vector(name: str, t, n: int, device: int):
-    import torch
     if t is None:
         raise Hb200Error(-5, f"{name}: null tensor")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise Hb200Error(-4, f"{name}: on {t.device}, the handle lives on cuda:{device}")
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] < n or (t.shape[0] > 1 and t.stride(0) != 1):
-        raise Hb200Error(-4, f"{name}: {t.dtype} {tuple(t.shape)}, strides {t.stride()} where {n} adjacent float32 values are wanted")
-    return C.c_void_p(t.data_ptr())
+    shape = t.shape
+    if t.dtype is not _F32 or len(shape) != 1 or shape[0] < n or (shape[0] > 1 and t.stride(0) != 1):
+        raise Hb200Error(-4, f"{name}: {t.dtype} {tuple(shape)}, strides {t.stride()} where {n} adjacent float32 values are wanted")
+    return t.data_ptr()
 
 
-def _i8_stream(stream, device: int) -> C.c_void_p:
-    if stream is None:
-        import torch
-        stream = torch.cuda.current_stream(device)
-    return C.c_void_p(int(stream.cuda_stream))
+def _i8_stream(stream, device: int) -> int:
+    return _raw_stream(device) if stream is None else stream.cuda_stream
 
 
 class WeightI8:
     """An int8 weight matrix with one f32 scale per row (output channel), resident on the device."""
 
     def __init__(self, handle):
+        _i8_torch()
         self._h = handle
         r, c, d = C.c_size_t(), C.c_size_t(), C.c_int()
         check(_l.load().hb200_weight_i8_info(self._h, C.byref(r), C.byref(c), None, C.byref(d)))
@@ -515,11 +524,11 @@ class WeightI8:
     @classmethod
     def upload_dev(cls, q_dev, scales_dev, stream=None):
         """CUDA tensors: int8 [n_rows, n_cols] (rows may be strided) and float32 [n_rows]."""
-        import torch
+        _i8_torch()
         if q_dev.dim() != 2:
             raise Hb200Error(-4, f"weights of shape {tuple(q_dev.shape)}: [n_rows, n_cols] is wanted")
         dev = q_dev.device.index
-        p, ld = _i8_rows("weights", q_dev, torch.int8, q_dev.shape[1], q_dev.shape[0], dev)
+        p, ld = _i8_rows("weights", q_dev, _I8, q_dev.shape[1], q_dev.shape[0], dev)
         s = _i8_vector("scales", scales_dev, q_dev.shape[0], dev)
         h = C.c_void_p()
         check(_l.load().hb200_weight_i8_upload_dev(q_dev.shape[0], q_dev.shape[1], p, ld, s, _i8_stream(stream, dev), C.byref(h)))
@@ -528,19 +537,18 @@ class WeightI8:
     @classmethod
     def quantize_dev(cls, w_dev, stream=None):
         """A float32 CUDA tensor [n_rows, n_cols], rounded to 8 bits row by row."""
-        import torch
+        _i8_torch()
         if w_dev.dim() != 2:
             raise Hb200Error(-4, f"weights of shape {tuple(w_dev.shape)}: [n_rows, n_cols] is wanted")
         dev = w_dev.device.index
-        p, ld = _i8_rows("weights", w_dev, torch.float32, w_dev.shape[1], w_dev.shape[0], dev)
+        p, ld = _i8_rows("weights", w_dev, _F32, w_dev.shape[1], w_dev.shape[0], dev)
         h = C.c_void_p()
         check(_l.load().hb200_weight_i8_quantize_dev(w_dev.shape[0], w_dev.shape[1], p, ld, _i8_stream(stream, dev), C.byref(h)))
         return cls(h)
 
     def store(self, q_dev=None, scales_dev=None, stream=None) -> None:
         """Row-major values and scales back into CUDA tensors (either may be None)."""
-        import torch
-        p, ld = _i8_rows("values", q_dev, torch.int8, self.n_cols, self.n_rows, self.device) if q_dev is not None else (None, 0)
+        p, ld = _i8_rows("values", q_dev, _I8, self.n_cols, self.n_rows, self.device) if q_dev is not None else (None, 0)
         s = _i8_vector("scales", scales_dev, self.n_rows, self.device) if scales_dev is not None else None
         check(_l.load().hb200_weight_i8_store_dev(self._h, p, ld, s, _i8_stream(stream, self.device)))
 
@@ -560,20 +568,23 @@ class ActI8:
     """Room for max_seq_len rows of n_cols int8 values with one f32 scale each, on the device."""
 
     def __init__(self, max_seq_len: int, n_cols: int):
+        _i8_torch()
         self._h = C.c_void_p()
         check(_l.load().hb200_act_i8_create(max_seq_len, n_cols, C.byref(self._h)))
         d = C.c_int()
-        check(_l.load().hb200_act_i8_info(self._h, None, None, C.byref(d)))
+        self._lib = _l.load()
+        check(self._lib.hb200_act_i8_info(self._h, None, None, C.byref(d)))
         self.max_seq_len, self.n_cols, self.device = max_seq_len, n_cols, int(d.value)
 
     def _f32(self, name, t, seq_len):
-        import torch
-        return _i8_rows(name, t, torch.float32, self.n_cols, seq_len, self.device)
+        return _i8_rows(name, t, _F32, self.n_cols, seq_len, self.device)
 
     def quantize(self, x_dev, seq_len: int, stream=None) -> None:
         """Float32 rows rounded to 8 bits, a scale per row (par_quantize, hearth-llm/src/pool.rs:467, has one per 32 columns)."""
         p, ld = self._f32("x", x_dev, seq_len)
-        check(_l.load().hb200_act_i8_quantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device)))
+        rc = self._lib.hb200_act_i8_quantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
+        if rc:
+            check(rc)
 
     def add_rms_norm(self, x_dev, weight_dev, eps: float, seq_len: int, residual_dev=None, sum_dev=None, stream=None) -> None:
         """h = x + residual (into sum_dev, which may be either of them), then weight * h / rms(h) rounded to 8 bits."""
@@ -589,7 +600,9 @@ class ActI8:
             if seq_len <= 1:
                 ld_s = ld
         w = _i8_vector("weight", weight_dev, self.n_cols, self.device)
-        check(_l.load().hb200_act_i8_add_rms_norm_dev(self._h, p, r, ld, w, eps, seq_len, s, ld_s, _i8_stream(stream, self.device)))
+        rc = self._lib.hb200_act_i8_add_rms_norm_dev(self._h, p, r, ld, w, eps, seq_len, s, ld_s, _i8_stream(stream, self.device))
+        if rc:
+            check(rc)
 
     def silu_mul(self, gate_dev, up_dev, seq_len: int, stream=None) -> None:
         """gate / (1 + exp(-gate)) * up rounded to 8 bits (ops::silu_mul_q8, hearth-llm/src/ops.rs:273, has a scale per 32 columns)."""
@@ -597,26 +610,28 @@ class ActI8:
         u, ld_u = self._f32("up", up_dev, seq_len)
         if seq_len > 1 and ld_u != ld:
             raise Hb200Error(-4, f"gate and up have rows {ld} and {ld_u} values apart: the same distance is wanted")
-        check(_l.load().hb200_act_i8_silu_mul_dev(self._h, g, u, ld, seq_len, _i8_stream(stream, self.device)))
+        rc = self._lib.hb200_act_i8_silu_mul_dev(self._h, g, u, ld, seq_len, _i8_stream(stream, self.device))
+        if rc:
+            check(rc)
 
     def load(self, q_dev, scales_dev, seq_len: int, stream=None) -> None:
         """Caller-made int8 rows and their scales."""
-        import torch
-        p, ld = _i8_rows("values", q_dev, torch.int8, self.n_cols, seq_len, self.device)
+        p, ld = _i8_rows("values", q_dev, _I8, self.n_cols, seq_len, self.device)
         s = _i8_vector("scales", scales_dev, seq_len, self.device)
         check(_l.load().hb200_act_i8_load_dev(self._h, p, ld, s, seq_len, _i8_stream(stream, self.device)))
 
     def store(self, q_dev, scales_dev, seq_len: int, stream=None) -> None:
         """Row-major int8 rows and scales back into CUDA tensors (either may be None)."""
-        import torch
-        p, ld = _i8_rows("values", q_dev, torch.int8, self.n_cols, seq_len, self.device) if q_dev is not None else (None, 0)
+        p, ld = _i8_rows("values", q_dev, _I8, self.n_cols, seq_len, self.device) if q_dev is not None else (None, 0)
         s = _i8_vector("scales", scales_dev, seq_len, self.device) if scales_dev is not None else None
         check(_l.load().hb200_act_i8_store_dev(self._h, p, ld, s, seq_len, _i8_stream(stream, self.device)))
 
     def dequantize(self, out_dev, seq_len: int, stream=None) -> None:
         """The float32 values the first seq_len rows stand for."""
         p, ld = self._f32("out", out_dev, seq_len)
-        check(_l.load().hb200_act_i8_dequantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device)))
+        rc = self._lib.hb200_act_i8_dequantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
+        if rc:
+            check(rc)
 
     def free(self) -> None:
         if self._h:
@@ -626,9 +641,10 @@ class ActI8:
 
 def matmul_i8_dev(w: WeightI8, a: ActI8, seq_len: int, out_dev, accumulate: bool = False, stream=None) -> None:
     """out[s][n] = or += sum_k(q_w q_x) * scale_w[n] * scale_x[s]; out_dev: float32 rows (strided if several products share them)."""
-    import torch
-    p, ld = _i8_rows("out", out_dev, torch.float32, w.n_rows, seq_len, w.device)
-    check(_l.load().hb200_matmul_i8_dev(w._h, a._h, seq_len, p, ld, 1 if accumulate else 0, _i8_stream(stream, w.device)))
+    p, ld = _i8_rows("out", out_dev, _F32, w.n_rows, seq_len, w.device)
+    rc = a._lib.hb200_matmul_i8_dev(w._h, a._h, seq_len, p, ld, 1 if accumulate else 0, _i8_stream(stream, w.device))
+    if rc:
+        check(rc)
 
 
 def matmul_i8(w: WeightI8, x: np.ndarray) -> np.ndarray:

@@ -37,6 +37,7 @@ struct DeviceScope {
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
         rc = use_slot_of(slot);
         if (rc) return;
+        if (prev == bound_device()) return;  // (use_slot_of may have switched, never away from the slot's device)
         const cudaError_t e = cudaSetDevice(bound_device());
         if (e != cudaSuccess) {
             set_error("cudaSetDevice(%d) failed: %s", bound_device(), cudaGetErrorString(e));
@@ -44,7 +45,7 @@ struct DeviceScope {
         }
     }
     ~DeviceScope() {
-        if (prev >= 0) cudaSetDevice(prev);
+        if (prev >= 0 && prev != bound_device()) cudaSetDevice(prev);
     }
 };
 

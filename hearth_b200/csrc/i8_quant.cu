@@ -69,40 +69,58 @@ __device__ __forceinline__ void write4(float* row, int c, int n, float4 v) {
 
 __device__ __forceinline__ float silu_mul1(float g, float u) { return __fmul_rn(__fdiv_rn(g, __fadd_rn(1.0f, expf(-g))), u); }
 
-// The four values v of columns c .. c + 3 (zero past the end); the norm adds h * h to `sq` and writes h.
-template <int OP, bool VEC>
-__device__ __forceinline__ float4 value4(const I8Rows& p, size_t row, int c, float& sq) {
-    const float4 x = read4<VEC>(p.x + row * p.ld, c, p.n_cols);
-    if (OP == I8_QUANTIZE) return x;
-    if (OP == I8_SILU_MUL) {
-        const float4 u = read4<VEC>(p.y + row * p.ld, c, p.n_cols);
-        return make_float4(silu_mul1(x.x, u.x), silu_mul1(x.y, u.y), silu_mul1(x.z, u.z), silu_mul1(x.w, u.w));
-    }
-    float4 h = x;
-    if (p.y) {
-        const float4 r = read4<VEC>(p.y + row * p.ld, c, p.n_cols);
-        h = make_float4(__fadd_rn(x.x, r.x), __fadd_rn(x.y, r.y), __fadd_rn(x.z, r.z), __fadd_rn(x.w, r.w));
-    }
-    if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols, h);
-    sq = fmaf(h.x, h.x, sq);
-    sq = fmaf(h.y, h.y, sq);
-    sq = fmaf(h.z, h.z, sq);
-    sq = fmaf(h.w, h.w, sq);
-    const float4 w = read4<VEC>(p.weight, c, p.n_cols);
-    return make_float4(__fmul_rn(w.x, h.x), __fmul_rn(w.y, h.y), __fmul_rn(w.z, h.z), __fmul_rn(w.w, h.w));
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+    return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
+}
+__device__ __forceinline__ float4 mul4(float4 a, float4 b) {
+    return make_float4(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y), __fmul_rn(a.z, b.z), __fmul_rn(a.w, b.w));
 }
 
-// The same values a second time, for rows that do not fit the registers: the norm reads h back where it was written
-// (x or r may be the same memory as the sum).
-template <int OP, bool VEC>
-__device__ __forceinline__ float4 value4_again(const I8Rows& p, size_t row, int c) {
-    if (OP == I8_ADD_RMS_NORM && p.sum) {
-        const float4 h = read4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols);
-        const float4 w = read4<VEC>(p.weight, c, p.n_cols);
-        return make_float4(__fmul_rn(w.x, h.x), __fmul_rn(w.y, h.y), __fmul_rn(w.z, h.z), __fmul_rn(w.w, h.w));
+// The values v of N float4s of a row, `step` columns apart from column c (zero past the end); the norm adds h * h to `sq`
+// and writes h.  All reads of the inputs come before the first write: the compiler may not move a read over a write
+// that could be to the same memory (the sum may overwrite an input), and reads one behind the other would leave HBM idle.
+template <int OP, bool VEC, int N>
+__device__ __forceinline__ void values(const I8Rows& p, size_t row, int c, int step, float4 (&v)[N], float& sq) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = read4<VEC>(p.x + row * p.ld, c + i * step, p.n_cols);
+    if (OP == I8_QUANTIZE) return;
+    if (OP == I8_ADD_RMS_NORM && !p.y) {
+        // h = x
+    } else {
+        float4 y[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i] = read4<VEC>(p.y + row * p.ld, c + i * step, p.n_cols);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (OP == I8_SILU_MUL)
+                v[i] = make_float4(silu_mul1(v[i].x, y[i].x), silu_mul1(v[i].y, y[i].y), silu_mul1(v[i].z, y[i].z), silu_mul1(v[i].w, y[i].w));
+            else
+                v[i] = add4(v[i], y[i]);
+        }
     }
+    if (OP == I8_SILU_MUL) return;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c + i * step, p.n_cols, v[i]);
+        sq = fmaf(v[i].x, v[i].x, sq);
+        sq = fmaf(v[i].y, v[i].y, sq);
+        sq = fmaf(v[i].z, v[i].z, sq);
+        sq = fmaf(v[i].w, v[i].w, sq);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = mul4(read4<VEC>(p.weight, c + i * step, p.n_cols), v[i]);
+}
+
+// One float4 a second time, for rows that do not fit the registers: the norm reads h back where it was written (x or r
+// may be the same memory as the sum).
+template <int OP, bool VEC>
+__device__ __forceinline__ float4 value_again(const I8Rows& p, size_t row, int c) {
+    if (OP == I8_ADD_RMS_NORM && p.sum)
+        return mul4(read4<VEC>(p.weight, c, p.n_cols), read4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols));
     float unused = 0.f;
-    return value4<OP, VEC>(p, row, c, unused);
+    float4 v[1];
+    values<OP, VEC, 1>(p, row, c, 0, v, unused);
+    return v[0];
 }
 
 __device__ __forceinline__ uint32_t absmax4(uint32_t m, float4 v) {
@@ -119,25 +137,28 @@ __device__ __forceinline__ uint32_t round4(float4 v, float inv) {
 }
 
 // One CTA per row.  NV = float4s of the row a thread keeps (0: the row is read twice).
-template <int OP, int NV, bool VEC>
-__global__ void __launch_bounds__(1024) i8_rows_kernel(const I8Rows p) {
+template <int OP, int NV, bool VEC, int MAX_THREADS, int MIN_CTAS>
+__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8Rows p) {
     __shared__ uint32_t s_max[32];
     __shared__ float s_sq[32];
     const int row = blockIdx.x;
     const int step = blockDim.x * 4;
     pdl_trigger();
     pdl_wait();
-    float4 v[NV > 0 ? NV : 1];
+    constexpr int BATCH = NV >= 4 ? 4 : (NV > 0 ? NV : 1), BATCHES = NV > 0 ? NV / BATCH : 1;
+    float4 v[BATCHES][BATCH];
     uint32_t m = 0;
     float sq = 0.f;
     if (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            v[i] = value4<OP, VEC>(p, row, threadIdx.x * 4 + i * step, sq);
-            m = absmax4(m, v[i]);
-        }
+        for (int b = 0; b < BATCHES; b++) values<OP, VEC, BATCH>(p, row, threadIdx.x * 4 + b * BATCH * step, step, v[b], sq);
+#pragma unroll
+        for (int i = 0; i < NV; i++) m = absmax4(m, v[i / BATCH][i % BATCH]);
     } else {
-        for (int c = threadIdx.x * 4; c < p.n_cols; c += step) m = absmax4(m, value4<OP, VEC>(p, row, c, sq));
+        for (int c = threadIdx.x * 4; c < p.n_cols; c += step) {
+            values<OP, VEC, BATCH>(p, row, c, 0, v[0], sq);
+            m = absmax4(m, v[0][0]);
+        }
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if (OP == I8_ADD_RMS_NORM) {
@@ -171,11 +192,11 @@ __global__ void __launch_bounds__(1024) i8_rows_kernel(const I8Rows p) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = threadIdx.x * 4 + i * step;
-            if (c < padded) *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(v[i], inv);
+            if (c < padded) *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(v[i / BATCH][i % BATCH], inv);
         }
     } else {
         for (int c = threadIdx.x * 4; c < padded; c += step)
-            *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(value4_again<OP, VEC>(p, row, c), inv);
+            *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(value_again<OP, VEC>(p, row, c), inv);
     }
 }
 
@@ -223,28 +244,39 @@ __global__ void __launch_bounds__(128) i8_store_kernel(I8Plane plane, const floa
     }
 }
 
-// Plane -> the f32 values it stands for, q * scale.
+// Plane -> the f32 values it stands for, q * scale.  A thread takes four columns of a group of eight rows: its eight loads
+// are in flight together (one row a thread ran at 2.4 TB/s).
 template <bool VEC>
 __global__ void __launch_bounds__(128) i8_dequantize_kernel(I8Plane plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld) {
     pdl_trigger();
     pdl_wait();
     const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
     if (c >= n_cols) return;
-    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(plane.q + plane_off(plane, row, c));
-        const float s = scales[row];
-        const float4 f = make_float4(__fmul_rn((float)(int8_t)(v), s), __fmul_rn((float)(int8_t)(v >> 8), s),
-                                     __fmul_rn((float)(int8_t)(v >> 16), s), __fmul_rn((float)(int8_t)(v >> 24), s));
-        write4<VEC>(out + (size_t)row * ld, c, n_cols, f);
+    const int row0 = blockIdx.y * 8, rows = min(8, n_rows - row0);
+    uint32_t v[8];
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = row0 + min(i, rows - 1);
+        v[i] = *reinterpret_cast<const uint32_t*>(plane.q + plane_off(plane, r, c));
+        s[i] = scales[r];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (i >= rows) break;
+        const float4 f = make_float4(__fmul_rn((float)(int8_t)(v[i]), s[i]), __fmul_rn((float)(int8_t)(v[i] >> 8), s[i]),
+                                     __fmul_rn((float)(int8_t)(v[i] >> 16), s[i]), __fmul_rn((float)(int8_t)(v[i] >> 24), s[i]));
+        write4<VEC>(out + (size_t)(row0 + i) * ld, c, n_cols, f);
     }
 }
 
 bool vec_rows(const void* p, size_t ld) { return ((reinterpret_cast<uintptr_t>(p) & 15) == 0) && (ld % 4 == 0); }
 
-template <int OP, int NV>
-int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStream_t st) {
+// A launch that may start its prologue under the end of the kernel before it.
+template <typename... P, typename... A>
+int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(n_rows);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -252,26 +284,32 @@ int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStrea
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    HB_CUDA(vec ? cudaLaunchKernelEx(&cfg, i8_rows_kernel<OP, NV, true>, p) : cudaLaunchKernelEx(&cfg, i8_rows_kernel<OP, NV, false>, p));
+    HB_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
     return 0;
+}
+
+template <int OP, int NV, int MAX_THREADS, int MIN_CTAS>
+int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStream_t st) {
+    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, MAX_THREADS, MIN_CTAS>, dim3(n_rows),
+                      threads, st, p);
 }
 
 template <int OP>
 int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
     const int quads = ((p.n_cols + 127) & ~127) / 4;  // float4s of a padded row
-    // Few rows: as many threads per row as there are float4s (latency).  Many rows: four float4s a thread, so that the
-    // loads of a row are in flight together and several rows share an SM.
-    const int want = n_rows >= 256 ? 4 : 1;
-    int nv = want;
-    while ((quads + nv - 1) / nv > 1024) nv *= 2;
-    if (nv > 8) return launch_rows_nv<OP, 0>(p, n_rows, 1024, vec, st);
-    const int threads = ((quads + nv - 1) / nv + 31) / 32 * 32;
-    switch (nv) {
-        case 1: return launch_rows_nv<OP, 1>(p, n_rows, threads, vec, st);
-        case 2: return launch_rows_nv<OP, 2>(p, n_rows, threads, vec, st);
-        case 4: return launch_rows_nv<OP, 4>(p, n_rows, threads, vec, st);
-        default: return launch_rows_nv<OP, 8>(p, n_rows, threads, vec, st);
-    }
+    const auto threads = [&](int nv) { return ((quads + nv - 1) / nv + 31) / 32 * 32; };
+    // Few rows: as few float4s a thread as still leave all rows resident at once (latency).  Many rows: four or eight, so
+    // that the loads of a row are in flight together and several rows share an SM, one computing while others load.
+    // Measured, us: silu_mul of 512 x 4096 5.2 with two, 7.7 with four; of 512 x 17408 20.4 with eight and two CTAs per SM,
+    // 35.3 with eight and one.
+    const auto resident = [&](int nv) { return threads(nv) <= 1024 && n_rows <= (long long)slot_sm_count() * (2048 / threads(nv)); };
+    if (resident(1)) return launch_rows_nv<OP, 1, 1024, 1>(p, n_rows, threads(1), vec, st);
+    if (resident(2)) return launch_rows_nv<OP, 2, 1024, 1>(p, n_rows, threads(2), vec, st);
+    if (threads(4) <= 512) return launch_rows_nv<OP, 4, 512, 2>(p, n_rows, threads(4), vec, st);
+    if (threads(4) <= 1024 && resident(4)) return launch_rows_nv<OP, 4, 1024, 1>(p, n_rows, threads(4), vec, st);
+    if (threads(8) <= 576) return launch_rows_nv<OP, 8, 576, 2>(p, n_rows, threads(8), vec, st);
+    if (threads(8) <= 1024) return launch_rows_nv<OP, 8, 1024, 1>(p, n_rows, threads(8), vec, st);
+    return launch_rows_nv<OP, 0, 1024, 1>(p, n_rows, 1024, vec, st);
 }
 
 dim3 move_grid(int n_rows, int n_cols) { return dim3((((n_cols + 127) & ~127) + 511) / 512, n_rows < 65535 ? n_rows : 65535); }
@@ -307,12 +345,9 @@ int launch_i8_store(const I8Plane& plane, const float* scales, int n_rows, int n
 
 int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld, cudaStream_t st) {
     if (n_rows <= 0) return 0;
-    if ((n_cols % 4 == 0) && vec_rows(out, ld))
-        i8_dequantize_kernel<true><<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, out, ld);
-    else
-        i8_dequantize_kernel<false><<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, out, ld);
-    HB_CUDA(cudaGetLastError());
-    return 0;
+    const dim3 grid((n_cols + 511) / 512, (n_rows + 7) / 8);
+    const bool vec = (n_cols % 4 == 0) && vec_rows(out, ld);
+    return launch_pdl(vec ? i8_dequantize_kernel<true> : i8_dequantize_kernel<false>, grid, 128, st, plane, scales, n_rows, n_cols, out, ld);
 }
 
 }  // namespace hb200
