@@ -12,6 +12,10 @@
 // The weight copies of the first stages are issued before the wait on the previous kernel of the stream (programmatic
 // dependent launch): weights are written once, at upload, which synchronises.
 //
+// Many tokens: bound by the tensor cores, so a pair of CTAs works on one tile of 256 rows x NT tokens (cta_group::2: each
+// SM holds half of either operand, which halves the shared-memory traffic per product), persistent over the tiles, two
+// accumulators in TMEM so that one tile is scaled and stored while the next is summed.
+//
 // Every wait on an mbarrier is bounded; on expiry the CTA records a status code, drains its copies, frees its TMEM and
 // returns (its cluster neighbours still meet it at the cluster barriers).
 #include <algorithm>
@@ -51,6 +55,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
+// True in one lane of a converged warp.  The roles below run their loops with the whole warp and elect a lane only around
+// the issuing instructions: inside a branch on the lane number those (their operands are warp-uniform registers) and
+// the barrier tests cost several times as much.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "elect.sync _|P, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -63,6 +79,17 @@ __device__ __forceinline__ int4 peer_ld4(uint32_t addr) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
+}
+
+// mbar_wait by a converged warp, whose lanes leave it together and agree on the answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if ((i & 7) == 7 && __any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    *abort_flag = 1;
+    atomicCAS(status, 0, code);
+    return false;
 }
 
 // The order of the two multiplications keeps an intermediate of tiny scales out of the subnormals.
@@ -91,7 +118,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     extern __shared__ unsigned char dyn[];
     __shared__ uint64_t full[STAGES], empty[STAGES], done;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, failed;
     __shared__ float s_sx[NTOK];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = gridDim.x, rank = blockIdx.x;
@@ -110,7 +137,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
             mbar_init(smem_u32(&empty[s]), 1);
         }
         mbar_init(smem_u32(&done), 1);
-        abort_flag = 0;
+        abort_flag = failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (int i = 0; i < nk && i < STAGES; i++) {
             mbar_expect_tx(smem_u32(&full[i]), W_TILE + x_bytes);
@@ -128,47 +155,50 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     pdl_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one())
             for (int i = 0; i < nk && i < STAGES; i++)
                 bulk_load(ring + i * C::STAGE + W_TILE, xp + (size_t)i * p.a_kb_stride, x_bytes, smem_u32(&full[i]));
-            int issued = min(nk, STAGES);
-            for (int i = STAGES; i < nk; i++) {
-                const int s = i % STAGES;
-                if (!mbar_wait(smem_u32(&empty[s]), (uint32_t)(i / STAGES - 1) & 1u, &abort_flag, p.status, 60)) break;
-                const uint32_t dst = ring + s * C::STAGE;
+        __syncwarp();
+        int issued = min(nk, STAGES);
+        for (int i = STAGES; i < nk; i++) {
+            const int s = i % STAGES;
+            if (!mbar_wait_warp(smem_u32(&empty[s]), (uint32_t)(i / STAGES - 1) & 1u, &abort_flag, p.status, 60)) break;
+            const uint32_t dst = ring + s * C::STAGE;
+            if (elect_one()) {
                 mbar_expect_tx(smem_u32(&full[s]), W_TILE + x_bytes);
                 bulk_load(dst, wp + (size_t)i * W_TILE, W_TILE, smem_u32(&full[s]));
                 bulk_load(dst + W_TILE, xp + (size_t)i * p.a_kb_stride, x_bytes, smem_u32(&full[s]));
-                issued = i + 1;
             }
-            if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
-                for (int i = max(0, issued - STAGES); i < issued; i++)
-                    for (uint32_t t = 0; t < SPIN_LIMIT && !mbar_try(smem_u32(&full[i % STAGES]), (uint32_t)(i / STAGES) & 1u); t++) {}
-            }
+            __syncwarp();
+            issued = i + 1;
+        }
+        if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
+            for (int i = max(0, issued - STAGES); i < issued; i++)
+                for (uint32_t t = 0; t < SPIN_LIMIT && !mbar_try(smem_u32(&full[i % STAGES]), (uint32_t)(i / STAGES) & 1u); t++) {}
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int i = 0; i < nk && ok; i++) {
-                const int s = i % STAGES;
-                ok = mbar_wait(smem_u32(&full[s]), (uint32_t)(i / STAGES) & 1u, &abort_flag, p.status, 61);
-                if (!ok) break;
-                tc_fence_after();
+        for (int i = 0; i < nk; i++) {
+            const int s = i % STAGES;
+            if (!mbar_wait_warp(smem_u32(&full[s]), (uint32_t)(i / STAGES) & 1u, &abort_flag, p.status, 61)) break;
+            tc_fence_after();
+            if (elect_one()) {
                 const uint64_t ad = make_desc(ring + s * C::STAGE), bd = make_desc(ring + s * C::STAGE + W_TILE);
 #pragma unroll
                 for (int j = 0; j < 4; j++) mma_i8(tmem, ad + 2 * j, bd + 2 * j, idesc_i8<NTOK>(), (i | j) != 0);
                 tc_commit(smem_u32(&empty[s]));
+                if (i == nk - 1) tc_commit(smem_u32(&done));
             }
-            tc_commit(smem_u32(&done));
+            __syncwarp();
         }
+        if (!mbar_wait_warp(smem_u32(&done), 0, &abort_flag, p.status, 62)) failed = 1;
         __syncwarp();
     } else if (warp == 2) {
         for (int t = lane; t < NTOK; t += 32) s_sx[t] = t < n_tok ? p.sx[tok0 + t] : 0.f;
     }
-    const bool ok = mbar_wait(smem_u32(&done), 0, &abort_flag, p.status, 62);
     __syncthreads();
     tc_fence_after();
+    const bool ok = !failed;
 
     const int row = row0 + warp * 32 + lane;
     const uint32_t tm = tmem + ((uint32_t)(warp * 32) << 16);
@@ -238,8 +268,256 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     }
 }
 
+// ---- a pair of CTAs per tile: many tokens ---------------------------------------------------------------------------
+
+template <int NT>
+struct PairCfg {
+    static constexpr int X_TILE = NT / 2 * 128;  // this CTA's half of the tokens
+    static constexpr int STAGE = W_TILE + X_TILE;
+    static constexpr int STAGES = NT == 256 ? 6 : 8;
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr uint32_t COLS = 2 * NT;  // two accumulators
+};
+constexpr int PAIR_THREADS = 192;  // producer, MMA issue (or relay), four epilogue warps
+// Token tiles that are walked together: their activations stay in L2 while the weights go by (16 x 256 tokens of
+// 17408 columns are 71 MB), and the weights are read once per group.
+constexpr int TOK_GROUP = 16;
+
+// Arrival at a barrier of the other CTA.  Neither side needs a fence for plain memory (with .release / .acquire.cluster on
+// this pair a stage took a microsecond): what the barrier orders are bulk copies and tensor-core reads of shared
+// memory, and TMEM reads, which tcgen05.fence covers.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives at the barrier of this offset in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+        "%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+struct PairTile {
+    int row_tile, tok0;  // this CTA's 128-row tile, first token of the pair's tile
+};
+// Tiles in groups of TOK_GROUP token tiles, the token tile fastest inside a group.
+template <int NT>
+__device__ __forceinline__ PairTile pair_tile(int t, int row_pairs, int tok_tiles, int rank) {
+    const int group = t / (TOK_GROUP * row_pairs), first = group * TOK_GROUP;
+    const int width = min(TOK_GROUP, tok_tiles - first), i = t - first * row_pairs;
+    PairTile r;
+    r.tok0 = (first + i % width) * NT;
+    r.row_tile = (i / width) * 2 + rank;
+    return r;
+}
+
+template <int NT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_pair_kernel(const I8Product p, int row_pairs, int tok_tiles) {
+    using C = PairCfg<NT>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ unsigned char dyn[];
+    // full: this CTA's copies of a stage; peer_full (leader): the other CTA's; empty: the stage may be refilled;
+    // acc_full / acc_empty: an accumulator is complete / has been read (leader: by both CTAs' epilogue warps)
+    __shared__ uint64_t full[STAGES], peer_full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, n_tiles = row_pairs * tok_tiles;
+    const int last_row_tile = (p.n_rows + 127) / 128 - 1;
+    const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u;
+
+    // What stage `it` of this CTA holds: weights and tokens of block k of tile t, and their bytes.
+    const auto x_bytes = [&](int tok0) {
+        const int left = p.n_tok - (tok0 + (int)rank * (NT / 2));
+        return left <= 0 ? 0u : (uint32_t)((min(left, NT / 2) + 7) / 8) * 1024u;
+    };
+    const auto w_src = [&](const PairTile& t, int k) { return p.w + ((size_t)min(t.row_tile, last_row_tile) * p.kb + k) * W_TILE; };
+    const auto x_src = [&](const PairTile& t, int k) { return p.a + (size_t)k * p.a_kb_stride + (size_t)(t.tok0 + (int)rank * (NT / 2)) * 128; };
+
+    pdl_trigger();
+    const PairTile t0 = pair_tile<NT>(pair, row_pairs, tok_tiles, rank);
+    const int ahead = min(p.kb, STAGES);  // stages whose weights are fetched before the wait on the previous kernel
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&peer_full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(smem_u32(&acc_full[a]), 1);
+            mbar_init(smem_u32(&acc_empty[a]), 8);
+        }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int k = 0; k < ahead; k++) {
+            mbar_expect_tx(smem_u32(&full[k]), W_TILE + x_bytes(t0.tok0));
+            bulk_load(ring + k * C::STAGE, w_src(t0, k), W_TILE, smem_u32(&full[k]));
+        }
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();  // both CTAs' barriers exist before either signals the other
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+
+    if (warp == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; t < n_tiles && ok; t += pairs) {
+            const PairTile tl = pair_tile<NT>(t, row_pairs, tok_tiles, rank);
+            const uint32_t xb = x_bytes(tl.tok0);
+            for (int k = 0; k < p.kb; k++, it++) {
+                const int s = it % STAGES;
+                const uint32_t dst = ring + s * C::STAGE, bar = smem_u32(&full[s]);
+                if (it >= STAGES) ok = mbar_wait_warp(smem_u32(&empty[s]), (uint32_t)(it / STAGES - 1) & 1u, &abort_flag, p.status, 63);
+                if (!ok) break;
+                if (elect_one()) {
+                    if (it >= ahead) {
+                        mbar_expect_tx(bar, W_TILE + xb);
+                        bulk_load(dst, w_src(tl, k), W_TILE, bar);
+                    }
+                    if (xb) bulk_load(dst + W_TILE, x_src(tl, k), xb, bar);
+                }
+                __syncwarp();
+            }
+        }
+        if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
+            for (int i = max(0, it - STAGES); i < it; i++)
+                for (uint32_t n = 0; n < SPIN_LIMIT && !mbar_try(smem_u32(&full[i % STAGES]), (uint32_t)(i / STAGES) & 1u); n++) {}
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // D = S32, A and B signed int8, both K-major, M = 256 over the pair, N = NT
+        constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int t = pair; t < n_tiles && ok; t += pairs, n++) {
+            const int a = n & 1;
+            if (rank == 0 && n >= 2) {
+                ok = mbar_wait_warp(smem_u32(&acc_empty[a]), (uint32_t)(n / 2 - 1) & 1u, &abort_flag, p.status, 64);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            for (int k = 0; k < p.kb; k++, it++) {
+                const int s = it % STAGES;
+                const uint32_t parity = (uint32_t)(it / STAGES) & 1u;
+                ok = mbar_wait_warp(smem_u32(&full[s]), parity, &abort_flag, p.status, 65);
+                if (!ok) break;
+                if (rank != 0) {  // tell the leader that this half of the stage has landed
+                    if (elect_one()) mbar_arrive_remote(peer_smem(smem_u32(&peer_full[s]), 0));
+                    __syncwarp();
+                    continue;
+                }
+                ok = mbar_wait_warp(smem_u32(&peer_full[s]), parity, &abort_flag, p.status, 66);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t ad = make_desc(ring + s * C::STAGE), bd = make_desc(ring + s * C::STAGE + W_TILE);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
+                    commit_pair(smem_u32(&empty[s]));
+                    if (k == p.kb - 1) commit_pair(smem_u32(&acc_full[a]));
+                }
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;  // TMEM lane quarter of this warp
+        const uint32_t leader_empty[2] = {peer_smem(smem_u32(&acc_empty[0]), 0), peer_smem(smem_u32(&acc_empty[1]), 0)};
+        int n = 0;
+        for (int t = pair; t < n_tiles; t += pairs, n++) {
+            const int a = n & 1;
+            const PairTile tl = pair_tile<NT>(t, row_pairs, tok_tiles, rank);
+            const int row = tl.row_tile * 128 + q * 32 + lane;
+            const bool live = row < p.n_rows;
+            const float sw = live ? p.sw[row] : 0.f;
+            if (!mbar_wait_warp(smem_u32(&acc_full[a]), (uint32_t)(n / 2) & 1u, &abort_flag, p.status, 67)) break;
+            tc_fence_after();
+            const uint32_t tm = tmem + a * NT + ((uint32_t)(q * 32) << 16);
+            const int n_tok = min(NT, p.n_tok - tl.tok0);
+            float* out = p.out + (size_t)tl.tok0 * p.ld_out + row;
+            for (int c0 = 0; c0 < n_tok; c0 += 32) {
+                uint32_t v[32];
+                const float sx = c0 + lane < n_tok ? p.sx[tl.tok0 + c0 + lane] : 0.f;
+                tmem_ld32(tm + c0, v);
+                float* o = out + (size_t)c0 * p.ld_out;
+                const int cols = min(32, n_tok - c0);
+                if (p.accumulate) {
+                    float b[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) b[j] = live && j < cols ? o[(size_t)j * p.ld_out] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float r = __fadd_rn(b[j], scaled((int)v[j], sw, __shfl_sync(0xffffffffu, sx, j)));
+                        if (live && j < cols) __stcs(o + (size_t)j * p.ld_out, r);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float r = scaled((int)v[j], sw, __shfl_sync(0xffffffffu, sx, j));
+                        if (live && j < cols) __stcs(o + (size_t)j * p.ld_out, r);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(leader_empty[a]);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    cluster_sync();  // the other CTA may still read this one's operands or signal its barriers
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+    }
+}
+
+template <int NT>
+int launch_pair(const I8Product& p, int sm_count, cudaStream_t st) {
+    const int row_pairs = (p.n_rows + 255) / 256, tok_tiles = (p.n_tok + NT - 1) / NT;
+    const long long tiles = (long long)row_pairs * tok_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count / 2));
+    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.dynamicSmemBytes = PairCfg<NT>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA(cudaLaunchKernelEx(&cfg, i8_pair_kernel<NT>, p, row_pairs, tok_tiles));
+    return 0;
+}
+
 struct Plan {
-    int ntok, split;
+    int ntok, split;  // split 0: the pair kernel
 };
 
 int g_sm_count = 148;
@@ -247,6 +525,7 @@ int g_sm_count = 148;
 int ntok_of(int n_tok) { return n_tok <= 16 ? 16 : n_tok <= 32 ? 32 : n_tok <= 64 ? 64 : n_tok <= 128 ? 128 : 256; }
 
 Plan plan(int n_rows, int kb, int n_tok) {
+    if (n_tok > 256) return {n_tok > 512 ? 256 : 128, 0};
     Plan best = {ntok_of(n_tok), 1};
     const long long tiles = (long long)((n_rows + 127) / 128) * ((n_tok + best.ntok - 1) / best.ntok);
     const int slots = g_sm_count * (best.ntok <= 128 ? 2 : 1);
@@ -288,11 +567,14 @@ int i8_gemm_prepare(int sm_count) {
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<64>::SMEM));
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<128>::SMEM));
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<256>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
     return 0;
 }
 
 int launch_i8_gemm(const I8Product& p, cudaStream_t st) {
     const Plan pl = plan(p.n_rows, p.kb, p.n_tok);
+    if (pl.split == 0) return pl.ntok == 256 ? launch_pair<256>(p, g_sm_count, st) : launch_pair<128>(p, g_sm_count, st);
     switch (pl.ntok) {
         case 16: return launch_split<16>(p, pl.split, st);
         case 32: return launch_split<32>(p, pl.split, st);
@@ -304,6 +586,7 @@ int launch_i8_gemm(const I8Product& p, cudaStream_t st) {
 
 const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok) {
     const Plan pl = plan(n_rows, kb, n_tok);
+    if (pl.split == 0) return pl.ntok == 256 ? "i8_tcgen05_pair_n256" : "i8_tcgen05_pair_n128";
     switch (pl.ntok) {
         case 16: return pl.split > 1 ? "i8_tcgen05_n16_split" : "i8_tcgen05_n16";
         case 32: return pl.split > 1 ? "i8_tcgen05_n32_split" : "i8_tcgen05_n32";
