@@ -346,6 +346,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     const int last_row_tile = (p.n_rows + 127) / 128 - 1;
     const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u;
 
+    const uint32_t full0 = smem_u32(&full[0]), peer0 = smem_u32(&peer_full[0]), empty0 = smem_u32(&empty[0]);
+
     // What stage `it` of this CTA holds: weights and tokens of block k of tile t, and their bytes.
     const auto x_bytes = [&](int tok0) {
         const int left = p.n_tok - (tok0 + (int)rank * (NT / 2));
@@ -385,35 +387,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     pdl_wait();
 
     if (warp == 0) {
-        int it = 0;
+        int it = 0, s = 0;
+        uint32_t phase = 1;  // parity of the `empty` completion before the one this use makes
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += pairs) {
             const PairTile tl = pair_tile<NT>(t, row_pairs, tok_tiles, rank);
             const uint32_t xb = x_bytes(tl.tok0);
+            const int8_t *ws = w_src(tl, 0), *xs = x_src(tl, 0);
             for (int k = 0; k < p.kb; k++, it++) {
-                const int s = it % STAGES;
-                const uint32_t dst = ring + s * C::STAGE, bar = smem_u32(&full[s]);
-                if (it >= STAGES) ok = mbar_wait_warp(smem_u32(&empty[s]), (uint32_t)(it / STAGES - 1) & 1u, &abort_flag, p.status, 63);
+                if (it >= STAGES) ok = mbar_wait_warp(empty0 + s * 8, phase, &abort_flag, p.status, 63);
                 if (!ok) break;
                 if (elect_one()) {
+                    const uint32_t dst = ring + s * C::STAGE, bar = full0 + s * 8;
                     if (it >= ahead) {
                         mbar_expect_tx(bar, W_TILE + xb);
-                        bulk_load(dst, w_src(tl, k), W_TILE, bar);
+                        bulk_load(dst, ws, W_TILE, bar);
                     }
-                    if (xb) bulk_load(dst + W_TILE, x_src(tl, k), xb, bar);
+                    if (xb) bulk_load(dst + W_TILE, xs, xb, bar);
                 }
                 __syncwarp();
+                ws += W_TILE;
+                xs += p.a_kb_stride;
+                if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
         if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
             for (int i = max(0, it - STAGES); i < it; i++)
-                for (uint32_t n = 0; n < SPIN_LIMIT && !mbar_try(smem_u32(&full[i % STAGES]), (uint32_t)(i / STAGES) & 1u); n++) {}
+                for (uint32_t n = 0; n < SPIN_LIMIT && !mbar_try(full0 + i % STAGES * 8, (uint32_t)(i / STAGES) & 1u); n++) {}
         }
         __syncwarp();
     } else if (warp == 1) {
         // D = S32, A and B signed int8, both K-major, M = 256 over the pair, N = NT
         constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-        int it = 0, n = 0;
+        const uint64_t ad0 = make_desc(ring), bd0 = make_desc(ring + W_TILE);
+        const uint32_t leader_full0 = peer_smem(smem_u32(&peer_full[0]), 0);
+        int n = 0, s = 0;
+        uint32_t phase = 0;
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += pairs, n++) {
             const int a = n & 1;
@@ -422,27 +431,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
                 if (!ok) break;
                 tc_fence_after();
             }
-            for (int k = 0; k < p.kb; k++, it++) {
-                const int s = it % STAGES;
-                const uint32_t parity = (uint32_t)(it / STAGES) & 1u;
-                ok = mbar_wait_warp(smem_u32(&full[s]), parity, &abort_flag, p.status, 65);
+            for (int k = 0; k < p.kb; k++) {
+                ok = mbar_wait_warp(full0 + s * 8, phase, &abort_flag, p.status, 65);
                 if (!ok) break;
                 if (rank != 0) {  // tell the leader that this half of the stage has landed
-                    if (elect_one()) mbar_arrive_remote(peer_smem(smem_u32(&peer_full[s]), 0));
+                    if (elect_one()) mbar_arrive_remote(leader_full0 + s * 8);
                     __syncwarp();
-                    continue;
-                }
-                ok = mbar_wait_warp(smem_u32(&peer_full[s]), parity, &abort_flag, p.status, 66);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t ad = make_desc(ring + s * C::STAGE), bd = make_desc(ring + s * C::STAGE + W_TILE);
+                } else {
+                    ok = mbar_wait_warp(peer0 + s * 8, phase, &abort_flag, p.status, 66);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t ad = ad0 + (uint32_t)(s * (C::STAGE >> 4)), bd = bd0 + (uint32_t)(s * (C::STAGE >> 4));
 #pragma unroll
-                    for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
-                    commit_pair(smem_u32(&empty[s]));
-                    if (k == p.kb - 1) commit_pair(smem_u32(&acc_full[a]));
+                        for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
+                        commit_pair(empty0 + s * 8);
+                        if (k == p.kb - 1) commit_pair(smem_u32(&acc_full[a]));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
         __syncwarp();
