@@ -273,8 +273,11 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
 template <int NT>
 struct PairCfg {
     static constexpr int X_TILE = NT / 2 * 128;  // this CTA's half of the tokens
-    static constexpr int STAGE = W_TILE + X_TILE;
-    static constexpr int STAGES = NT == 256 ? 6 : 8;
+    // Two 128-column blocks a stage (the last stage of a tile may hold one): a barrier test costs the issuing warp some
+    // 160 cycles even when it succeeds, and a stage has two of them; with one block a stage (256 cycles of MMAs at 128
+    // tokens) the tensor pipe waited for the issue.
+    static constexpr int STAGE = 2 * (W_TILE + X_TILE);
+    static constexpr int STAGES = NT == 256 ? 3 : 4;
     static constexpr int SMEM = STAGES * STAGE + 1024;
     static constexpr uint32_t COLS = 2 * NT;  // two accumulators
 };
@@ -353,12 +356,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         const int left = p.n_tok - (tok0 + (int)rank * (NT / 2));
         return left <= 0 ? 0u : (uint32_t)((min(left, NT / 2) + 7) / 8) * 1024u;
     };
-    const auto w_src = [&](const PairTile& t, int k) { return p.w + ((size_t)min(t.row_tile, last_row_tile) * p.kb + k) * W_TILE; };
-    const auto x_src = [&](const PairTile& t, int k) { return p.a + (size_t)k * p.a_kb_stride + (size_t)(t.tok0 + (int)rank * (NT / 2)) * 128; };
+    const auto w_src = [&](const PairTile& t) { return p.w + (size_t)min(t.row_tile, last_row_tile) * p.kb * W_TILE; };
+    const auto x_src = [&](const PairTile& t) { return p.a + (size_t)(t.tok0 + (int)rank * (NT / 2)) * 128; };
 
     pdl_trigger();
     const PairTile t0 = pair_tile<NT>(pair, row_pairs, tok_tiles, rank);
-    const int ahead = min(p.kb, STAGES);  // stages whose weights are fetched before the wait on the previous kernel
+    const int steps = (p.kb + 1) / 2;     // stages of a tile
+    const int ahead = min(steps, STAGES);  // stages whose weights are fetched before the wait on the previous kernel
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full[s]), 1);
@@ -372,8 +376,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (int k = 0; k < ahead; k++) {
-            mbar_expect_tx(smem_u32(&full[k]), W_TILE + x_bytes(t0.tok0));
-            bulk_load(ring + k * C::STAGE, w_src(t0, k), W_TILE, smem_u32(&full[k]));
+            const uint32_t blocks = min(2, p.kb - 2 * k);
+            mbar_expect_tx(full0 + k * 8, blocks * (W_TILE + x_bytes(t0.tok0)));
+            bulk_load(ring + k * C::STAGE, w_src(t0) + (size_t)k * 2 * W_TILE, blocks * W_TILE, full0 + k * 8);
         }
     }
     if (warp == 1) {
@@ -393,21 +398,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         for (int t = pair; t < n_tiles && ok; t += pairs) {
             const PairTile tl = pair_tile<NT>(t, row_pairs, tok_tiles, rank);
             const uint32_t xb = x_bytes(tl.tok0);
-            const int8_t *ws = w_src(tl, 0), *xs = x_src(tl, 0);
-            for (int k = 0; k < p.kb; k++, it++) {
+            const int8_t *ws = w_src(tl), *xs = x_src(tl);
+            for (int k = 0; k < p.kb; k += 2, it++) {
                 if (it >= STAGES) ok = mbar_wait_warp(empty0 + s * 8, phase, &abort_flag, p.status, 63);
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t dst = ring + s * C::STAGE, bar = full0 + s * 8;
+                    const uint32_t blocks = min(2, p.kb - k);
                     if (it >= ahead) {
-                        mbar_expect_tx(bar, W_TILE + xb);
-                        bulk_load(dst, ws, W_TILE, bar);
+                        mbar_expect_tx(bar, blocks * (W_TILE + xb));
+                        bulk_load(dst, ws, blocks * W_TILE, bar);
                     }
-                    if (xb) bulk_load(dst + W_TILE, xs, xb, bar);
+                    if (xb) {
+                        bulk_load(dst + 2 * W_TILE, xs, xb, bar);
+                        if (blocks == 2) bulk_load(dst + 2 * W_TILE + C::X_TILE, xs + p.a_kb_stride, xb, bar);
+                    }
                 }
                 __syncwarp();
-                ws += W_TILE;
-                xs += p.a_kb_stride;
+                ws += 2 * W_TILE;
+                xs += 2 * p.a_kb_stride;
                 if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
@@ -419,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     } else if (warp == 1) {
         // D = S32, A and B signed int8, both K-major, M = 256 over the pair, N = NT
         constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-        const uint64_t ad0 = make_desc(ring), bd0 = make_desc(ring + W_TILE);
+        const uint64_t ad0 = make_desc(ring), bd0 = make_desc(ring + 2 * W_TILE);
         const uint32_t leader_full0 = peer_smem(smem_u32(&peer_full[0]), 0);
         int n = 0, s = 0;
         uint32_t phase = 0;
@@ -431,7 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
                 if (!ok) break;
                 tc_fence_after();
             }
-            for (int k = 0; k < p.kb; k++) {
+            for (int k = 0; k < p.kb; k += 2) {
                 ok = mbar_wait_warp(full0 + s * 8, phase, &abort_flag, p.status, 65);
                 if (!ok) break;
                 if (rank != 0) {  // tell the leader that this half of the stage has landed
@@ -445,8 +454,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
                         const uint64_t ad = ad0 + (uint32_t)(s * (C::STAGE >> 4)), bd = bd0 + (uint32_t)(s * (C::STAGE >> 4));
 #pragma unroll
                         for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
+                        if (k + 1 < p.kb) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                mma_i8_pair(tmem + a * NT, ad + (W_TILE >> 4) + 2 * j, bd + (C::X_TILE >> 4) + 2 * j, IDESC, 1);
+                        }
                         commit_pair(empty0 + s * 8);
-                        if (k == p.kb - 1) commit_pair(smem_u32(&acc_full[a]));
+                        if (k + 2 >= p.kb) commit_pair(smem_u32(&acc_full[a]));
                     }
                     __syncwarp();
                 }
