@@ -281,7 +281,8 @@ struct PairCfg {
     static constexpr int SMEM = STAGES * STAGE + 1024;
     static constexpr uint32_t COLS = 2 * NT;  // two accumulators
 };
-constexpr int PAIR_THREADS = 192;  // producer, MMA issue (or relay), four epilogue warps
+constexpr int PAIR_EPI_WARPS = 8;  // two per TMEM lane quarter, each half of the tile's tokens
+constexpr int PAIR_THREADS = 32 * (2 + PAIR_EPI_WARPS);  // producer, MMA issue (or relay), epilogue
 // Token tiles that are walked together: their activations stay in L2 while the weights go by (16 x 256 tokens of
 // 17408 columns are 71 MB), and the weights are read once per group.
 constexpr int TOK_GROUP = 16;
@@ -318,6 +319,27 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "memory");
 }
 
+// 32 tokens of a row: a warp's store is 32 neighbouring rows of one token.  The output of a long prompt is larger than L2
+// and not read back here: stored for early eviction.
+template <bool ACC, bool PART>
+__device__ __forceinline__ void store_cols(float* o, size_t ld, const uint32_t (&v)[32], float sw, float sx, bool live, int cols) {
+    float r[32];
+#pragma unroll
+    for (int j = 0; j < 32; j++) r[j] = scaled((int)v[j], sw, __shfl_sync(0xffffffffu, sx, j));
+    if (!live) return;
+    if (ACC) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (!PART || j < cols) r[j] = __fadd_rn(__ldcs(o + (size_t)j * ld), r[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+        if (PART && j >= cols) break;
+        __stcs(o, r[j]);
+        o += ld;
+    }
+}
+
 struct PairTile {
     int row_tile, tok0;  // this CTA's 128-row tile, first token of the pair's tile
 };
@@ -332,7 +354,7 @@ __device__ __forceinline__ PairTile pair_tile(int t, int row_pairs, int tok_tile
     return r;
 }
 
-template <int NT>
+template <int NT, bool ACC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_pair_kernel(const I8Product p, int row_pairs, int tok_tiles) {
     using C = PairCfg<NT>;
     constexpr int STAGES = C::STAGES;
@@ -371,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(smem_u32(&acc_full[a]), 1);
-            mbar_init(smem_u32(&acc_empty[a]), 8);
+            mbar_init(smem_u32(&acc_empty[a]), 2 * PAIR_EPI_WARPS);
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -469,7 +491,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         }
         __syncwarp();
     } else {
-        const int q = warp & 3;  // TMEM lane quarter of this warp
+        const int q = warp & 3;                      // TMEM lane quarter of this warp
+        const int half = (warp - 2) / 4 * (NT / 2);  // its first token of the tile
         const uint32_t leader_empty[2] = {peer_smem(smem_u32(&acc_empty[0]), 0), peer_smem(smem_u32(&acc_empty[1]), 0)};
         int n = 0;
         for (int t = pair; t < n_tiles; t += pairs, n++) {
@@ -480,30 +503,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
             const float sw = live ? p.sw[row] : 0.f;
             if (!mbar_wait_warp(smem_u32(&acc_full[a]), (uint32_t)(n / 2) & 1u, &abort_flag, p.status, 67)) break;
             tc_fence_after();
-            const uint32_t tm = tmem + a * NT + ((uint32_t)(q * 32) << 16);
-            const int n_tok = min(NT, p.n_tok - tl.tok0);
-            float* out = p.out + (size_t)tl.tok0 * p.ld_out + row;
+            const uint32_t tm = tmem + a * NT + half + ((uint32_t)(q * 32) << 16);
+            const int n_tok = min(NT / 2, p.n_tok - tl.tok0 - half);
+            const float* sxs = p.sx + tl.tok0 + half;
+            float* out = p.out + (size_t)(tl.tok0 + half) * p.ld_out + row;
             for (int c0 = 0; c0 < n_tok; c0 += 32) {
                 uint32_t v[32];
-                const float sx = c0 + lane < n_tok ? p.sx[tl.tok0 + c0 + lane] : 0.f;
+                const float sx = c0 + lane < n_tok ? sxs[c0 + lane] : 0.f;
                 tmem_ld32(tm + c0, v);
                 float* o = out + (size_t)c0 * p.ld_out;
-                const int cols = min(32, n_tok - c0);
-                if (p.accumulate) {
-                    float b[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) b[j] = live && j < cols ? o[(size_t)j * p.ld_out] : 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float r = __fadd_rn(b[j], scaled((int)v[j], sw, __shfl_sync(0xffffffffu, sx, j)));
-                        if (live && j < cols) __stcs(o + (size_t)j * p.ld_out, r);
-                    }
+                if (c0 + 32 <= n_tok) {
+                    store_cols<ACC, false>(o, p.ld_out, v, sw, sx, live, 32);
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float r = scaled((int)v[j], sw, __shfl_sync(0xffffffffu, sx, j));
-                        if (live && j < cols) __stcs(o + (size_t)j * p.ld_out, r);
-                    }
+                    store_cols<ACC, true>(o, p.ld_out, v, sw, sx, live, n_tok - c0);
                 }
             }
             tc_fence_before();
@@ -534,7 +546,7 @@ int launch_pair(const I8Product& p, int sm_count, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    HB_CUDA(cudaLaunchKernelEx(&cfg, i8_pair_kernel<NT>, p, row_pairs, tok_tiles));
+    HB_CUDA(cudaLaunchKernelEx(&cfg, p.accumulate ? i8_pair_kernel<NT, true> : i8_pair_kernel<NT, false>, p, row_pairs, tok_tiles));
     return 0;
 }
 
@@ -589,8 +601,10 @@ int i8_gemm_prepare(int sm_count) {
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<64>::SMEM));
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<128>::SMEM));
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<256>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
     return 0;
 }
 
