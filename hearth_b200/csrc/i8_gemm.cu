@@ -8,7 +8,7 @@
 //
 // Few tokens: the time is the weights' way from HBM, and what counts is how many bytes are in flight on how many SMs.
 // A tile of 128 rows is cut along K over the CTAs of a cluster; integer partial sums meet through distributed shared
-// memory (no workspace, no atomics, any order gives the same bits), every CTA finishing its share of the tile.
+// memory (no workspace, no atomics, any order gives the same bits), every CTA finishing its share of the tokens.
 // The weight copies of the first stages are issued before the wait on the previous kernel of the stream (programmatic
 // dependent launch): weights are written once, at upload, which synchronises.
 //
@@ -70,15 +70,15 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ int4 peer_ld4(uint32_t addr) {
-    int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void peer_st(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // mbar_wait by a converged warp, whose lanes leave it together and agree on the answer.
@@ -105,9 +105,14 @@ struct SplitCfg {
     static constexpr int X_TILE = NTOK * 128;
     static constexpr int STAGE = W_TILE + X_TILE;
     // two CTAs per SM up to 128 tokens
-    static constexpr int STAGES = NTOK <= 32 ? 5 : (NTOK <= 64 ? 4 : (NTOK <= 128 ? 3 : 4));
-    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int STAGES = NTOK <= 16 ? 5 : (NTOK <= 64 ? 4 : (NTOK <= 128 ? 3 : 4));
+    // Partial sums of the cluster's other CTAs: memory of their own at few tokens, else the ring's once it has run dry
+    // (`split` senders with ceil(NTOK / split) tokens of 128 rows each).
+    static constexpr bool OWN_PART = NTOK <= 32;
+    static constexpr int PART = (NTOK + MAX_SPLIT) * 512;
+    static constexpr int SMEM = STAGES * STAGE + (OWN_PART ? PART : 0) + 1024;
     static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
+    static_assert(OWN_PART || PART <= STAGES * STAGE, "partial sums fit the ring");
 };
 
 // grid (split, token tiles, row tiles), cluster (split, 1, 1): rank r of a cluster takes blocks [kb * r / split, kb * (r + 1) / split).
@@ -148,6 +153,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (C::OWN_PART && split > 1) cluster_arrive();  // this CTA runs: its memory may be written (awaited far below)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -217,26 +223,37 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
                 }
         }
     } else {
-        // partial sums of the tile, [token][128 rows], in the memory of the ring: every copy has landed and been read
-        int* part = reinterpret_cast<int*>(dyn + (ring - smem_u32(dyn)));
+        // Every CTA finishes its share of the tokens: the others store their sums of them into its memory, [sender][token]
+        // [128 rows] (stores do not wait for an answer; loads from the others took 6 000 cycles at 77 tokens).
+        const int share = (n_tok + split - 1) / split;
+        const uint32_t part = C::OWN_PART ? ring + STAGES * C::STAGE : ring;
+        const uint32_t mine = part + (uint32_t)(rank * share * 512 + (warp * 32 + lane) * 4);
+        if (!C::OWN_PART) cluster_arrive();  // this CTA's copies have landed and been read
+        cluster_wait();                      // the others' memory is there (and free)
         for (int c0 = 0; c0 < n_tok; c0 += 16) {
             uint32_t v[16];
             tmem_ld16(tm + c0, v);
+            int owner = c0 / share, at = c0 - owner * share;
+            uint32_t dst = peer_smem(mine, owner);
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (c0 + j < n_tok) part[(c0 + j) * 128 + warp * 32 + lane] = (int)v[j];
+            for (int j = 0; j < 16; j++) {
+                if (c0 + j < n_tok) peer_st(dst + at * 512, v[j]);
+                if (++at == share) { at = 0; owner++; dst = peer_smem(mine, min(owner, split - 1)); }
+            }
         }
         cluster_sync();
-        const int n_vec = n_tok * 32;
-        const int v0 = n_vec * rank / split, v1 = n_vec * (rank + 1) / split;
+        const int4* sums = reinterpret_cast<const int4*>(dyn + (part - smem_u32(dyn)));
+        const int n_mine = min(share, n_tok - rank * share);
         const bool vec = (p.ld_out % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0);
-        for (int i = v0 + tid; i < v1; i += 128) {
+        for (int i = tid; i < n_mine * 32; i += 128) {
             int4 s = make_int4(0, 0, 0, 0);
-            for (int r = 0; r < split; r++) {
-                const int4 t = peer_ld4(peer_smem(ring + i * 16, r));
-                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-            }
-            const int tok = i >> 5, r4 = row0 + (i & 31) * 4;
+#pragma unroll
+            for (int r = 0; r < MAX_SPLIT; r++)
+                if (r < split) {
+                    const int4 t = sums[r * share * 32 + i];
+                    s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+                }
+            const int tok = rank * share + (i >> 5), r4 = row0 + (i & 31) * 4;
             const float sx = s_sx[tok];
             float* o = p.out + (size_t)(tok0 + tok) * p.ld_out + r4;
             if (!ok) continue;
@@ -258,7 +275,6 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
                     }
             }
         }
-        cluster_sync();  // a neighbour may still be reading this CTA's partial sums
     }
     tc_fence_before();
     __syncthreads();
