@@ -104,8 +104,8 @@ template <int NTOK>
 struct SplitCfg {
     static constexpr int X_TILE = NTOK * 128;
     static constexpr int STAGE = W_TILE + X_TILE;
-    // two CTAs per SM up to 128 tokens
-    static constexpr int STAGES = NTOK <= 16 ? 5 : (NTOK <= 64 ? 4 : (NTOK <= 128 ? 3 : 4));
+    // two CTAs per SM
+    static constexpr int STAGES = NTOK <= 16 ? 5 : 4;
     // Partial sums of the cluster's other CTAs: memory of their own at few tokens, else the ring's once it has run dry
     // (`split` senders with ceil(NTOK / split) tokens of 128 rows each).
     static constexpr bool OWN_PART = NTOK <= 32;
@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, failed;
     __shared__ float s_sx[NTOK];
+    __shared__ alignas(16) float s_sw[128];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = gridDim.x, rank = blockIdx.x;
     const int tok0 = blockIdx.y * NTOK, row_tile = blockIdx.z, row0 = row_tile * 128;
@@ -153,7 +154,8 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (C::OWN_PART && split > 1) cluster_arrive();  // this CTA runs: its memory may be written (awaited far below)
+    // This CTA runs: its memory may be written (awaited far below).  Relaxed: a release would wait for the bulk copies.
+    if (C::OWN_PART && split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -201,6 +203,8 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
         __syncwarp();
     } else if (warp == 2) {
         for (int t = lane; t < NTOK; t += 32) s_sx[t] = t < n_tok ? p.sx[tok0 + t] : 0.f;
+    } else {
+        for (int r = lane; r < 128; r += 32) s_sw[r] = row0 + r < p.n_rows ? p.sw[row0 + r] : 0.f;
     }
     __syncthreads();
     tc_fence_after();
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     const int row = row0 + warp * 32 + lane;
     const uint32_t tm = tmem + ((uint32_t)(warp * 32) << 16);
     if (split == 1) {
-        const float sw = row < p.n_rows ? p.sw[row] : 0.f;
+        const float sw = s_sw[warp * 32 + lane];
         float* out = p.out + (size_t)tok0 * p.ld_out + row;
         for (int c0 = 0; c0 < n_tok; c0 += 16) {
             uint32_t v[16];
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
             float* o = p.out + (size_t)(tok0 + tok) * p.ld_out + r4;
             if (!ok) continue;
             if (vec && r4 + 3 < p.n_rows) {
-                const float4 w = *reinterpret_cast<const float4*>(p.sw + r4);
+                const float4 w = *reinterpret_cast<const float4*>(&s_sw[(i & 31) * 4]);
                 float4 f = make_float4(scaled(s.x, w.x, sx), scaled(s.y, w.y, sx), scaled(s.z, w.z, sx), scaled(s.w, w.w, sx));
                 if (p.accumulate) {
                     const float4 b = *reinterpret_cast<const float4*>(o);
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (r4 + j < p.n_rows) {
-                        const float f = scaled(q[j], p.sw[r4 + j], sx);
+                        const float f = scaled(q[j], s_sw[(i & 31) * 4 + j], sx);
                         o[j] = p.accumulate ? __fadd_rn(o[j], f) : f;
                     }
             }
@@ -571,40 +575,80 @@ struct Plan {
 };
 
 int g_sm_count = 148;
+// Clusters of the split kernel resident at once, by size: twice what the occupancy query says (it counts one CTA per SM,
+// two run).  These are a B200's, replaced by the device's own when the library is initialised.
+int g_clusters[MAX_SPLIT + 1] = {0, 296, 148, 90, 66, 52, 44, 30, 30};
 
-int ntok_of(int n_tok) { return n_tok <= 16 ? 16 : n_tok <= 32 ? 32 : n_tok <= 64 ? 64 : n_tok <= 128 ? 128 : 256; }
-
+// Which kernel, with which tile and how many CTAs along K.
+//   split   one token tile of 16, 32 or 64 where that covers the batch.  As many CTAs per tile as keep all clusters
+//           resident at once: measured, us, at 1 / 2 / 3 / 4 / 5 / 6 / 8 CTAs along K: 32 tokens of 17408 x 5120 (40 tiles)
+//           - / - / 19.3 / 17.8 / 17.2 / 16.5 / 22.3 (at 8 a part of the clusters waits), 16 of 4096 x 24576 (192 tiles)
+//           18.0 / 22.2 / 24.6 / 23.1 / 26.1.
+//   pair    from 65 tokens on where it is estimated to be faster.  The estimates (microseconds; fixed part, then the time
+//           of a 128-column block per wave of tiles, or the bytes read by the SMs) fit 128 x 4096 x 4096 (split 9.0, pair
+//           9.2), 77 x 12288 x 4096 (14.7, 25), 128 x 4096 x 24576 (30.8, 24.2), 200 x 4096 x 4096 (11.3, 9.5), 512 x 4096 x
+//           24576 (pair of 128 tokens 50, of 256 44.6) and 512 x 4096 x 4096 (11.6, 15.5) on the right side.
 Plan plan(int n_rows, int kb, int n_tok) {
-    if (n_tok > 256) return {n_tok > 512 ? 256 : 128, 0};
-    Plan best = {ntok_of(n_tok), 1};
-    const long long tiles = (long long)((n_rows + 127) / 128) * ((n_tok + best.ntok - 1) / best.ntok);
-    const int slots = g_sm_count * (best.ntok <= 128 ? 2 : 1);
-    double best_t = 1e30;
-    for (int s = 1; s <= MAX_SPLIT && s <= kb; s++) {
-        const long long waves = (tiles * s + slots - 1) / slots;
-        const double t = waves * ((kb + s - 1) / s + 2.0 + (s > 1 ? 1.0 : 0.0));
-        if (t < best_t) { best_t = t; best.split = s; }
+    Plan best = {n_tok <= 16 ? 16 : n_tok <= 32 ? 32 : 64, 1};
+    const long long row_tiles = (n_rows + 127) / 128, tiles = row_tiles * ((n_tok + best.ntok - 1) / best.ntok);
+    for (int s = 2; s <= MAX_SPLIT && 2 * s <= kb; s++)
+        if (tiles <= g_clusters[s]) best.split = s;
+    if (n_tok <= 64) return best;
+    const double hbm = ((double)row_tiles * kb * W_TILE + 4.0 * n_rows * n_tok) / 6.0e6;
+    double best_t = 5.0 + std::max((double)tiles * kb * (W_TILE + 64 * 128) / 13.0e6, hbm);
+    for (int nt = 128; nt <= 256; nt *= 2) {
+        const long long pairs = (long long)((n_rows + 255) / 256) * ((n_tok + nt - 1) / nt), at_once = g_sm_count / 2;
+        const double t = (nt == 128 ? 4.0 : 5.0) + std::max((double)((pairs + at_once - 1) / at_once) * kb * (nt == 128 ? 0.22 : 0.38), hbm);
+        if (t < best_t) { best_t = t; best = {nt, 0}; }
     }
     return best;
 }
 
 template <int NTOK>
-int launch_split(const I8Product& p, int split, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split, (p.n_tok + NTOK - 1) / NTOK, (p.n_rows + 127) / 128);
+void split_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], dim3 grid, cudaStream_t st) {
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = SplitCfg<NTOK>::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = split;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = grid.x;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
+}
+
+template <int NTOK>
+int launch_split(const I8Product& p, int split, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    split_config<NTOK>(cfg, attr, dim3(split, (p.n_tok + NTOK - 1) / NTOK, (p.n_rows + 127) / 128), st);
     HB_CUDA(cudaLaunchKernelEx(&cfg, i8_split_kernel<NTOK>, p));
+    return 0;
+}
+
+template <int NTOK>
+int prepare_split() {
+    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<NTOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<NTOK>::SMEM));
+    if (NTOK != 16) return 0;  // the others hold as much shared memory
+    for (int s = 2; s <= MAX_SPLIT; s++) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        split_config<NTOK>(cfg, attr, dim3(s, 1, 1), nullptr);
+        cfg.numAttrs = 1;
+        int n = 0;
+        HB_CUDA(cudaOccupancyMaxActiveClusters(&n, i8_split_kernel<NTOK>, &cfg));
+        g_clusters[s] = 2 * n;
+    }
+    return 0;
+}
+
+template <int NT>
+int prepare_pair() {
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<NT>::SMEM));
+    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<NT>::SMEM));
     return 0;
 }
 
@@ -612,16 +656,12 @@ int launch_split(const I8Product& p, int split, cudaStream_t st) {
 
 int i8_gemm_prepare(int sm_count) {
     g_sm_count = sm_count;
-    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<16>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<32>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<64>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<128>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<256>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<128>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
-    HB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<256>::SMEM));
-    return 0;
+    int rc;
+    if ((rc = prepare_split<16>())) return rc;
+    if ((rc = prepare_split<32>())) return rc;
+    if ((rc = prepare_split<64>())) return rc;
+    if ((rc = prepare_pair<128>())) return rc;
+    return prepare_pair<256>();
 }
 
 int launch_i8_gemm(const I8Product& p, cudaStream_t st) {
@@ -630,9 +670,7 @@ int launch_i8_gemm(const I8Product& p, cudaStream_t st) {
     switch (pl.ntok) {
         case 16: return launch_split<16>(p, pl.split, st);
         case 32: return launch_split<32>(p, pl.split, st);
-        case 64: return launch_split<64>(p, pl.split, st);
-        case 128: return launch_split<128>(p, pl.split, st);
-        default: return launch_split<256>(p, pl.split, st);
+        default: return launch_split<64>(p, pl.split, st);
     }
 }
 
@@ -642,9 +680,7 @@ const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok) {
     switch (pl.ntok) {
         case 16: return pl.split > 1 ? "i8_tcgen05_n16_split" : "i8_tcgen05_n16";
         case 32: return pl.split > 1 ? "i8_tcgen05_n32_split" : "i8_tcgen05_n32";
-        case 64: return pl.split > 1 ? "i8_tcgen05_n64_split" : "i8_tcgen05_n64";
-        case 128: return pl.split > 1 ? "i8_tcgen05_n128_split" : "i8_tcgen05_n128";
-        default: return pl.split > 1 ? "i8_tcgen05_n256_split" : "i8_tcgen05_n256";
+        default: return pl.split > 1 ? "i8_tcgen05_n64_split" : "i8_tcgen05_n64";
     }
 }
 

@@ -300,7 +300,7 @@ int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
     const auto threads = [&](int nv) { return ((quads + nv - 1) / nv + 31) / 32 * 32; };
     // Few rows: as few float4s a thread as still leave all rows resident at once (latency).  Many rows: four or eight, so
     // that the loads of a row are in flight together and several rows share an SM, one computing while others load.
-    // Measured, us: silu_mul of 512 x 4096 5.2 with two, 7.7 with four; of 512 x 17408 20.4 with eight and two CTAs per SM,
+    // Measured, us: silu_mul of 512 x 4096 4.7 with two, 7.7 with four; of 512 x 17408 20.4 with eight and two CTAs per SM,
     // 35.3 with eight and one.
     const auto resident = [&](int nv) { return threads(nv) <= 1024 && n_rows <= (long long)slot_sm_count() * (2048 / threads(nv)); };
     if (resident(1)) return launch_rows_nv<OP, 1, 1024, 1>(p, n_rows, threads(1), vec, st);
