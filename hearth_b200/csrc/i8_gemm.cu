@@ -632,16 +632,6 @@ int launch_split(const I8Product& p, int split, cudaStream_t st) {
 template <int NTOK>
 int prepare_split() {
     HB_CUDA(cudaFuncSetAttribute(i8_split_kernel<NTOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<NTOK>::SMEM));
-    if (NTOK != 16) return 0;  // the others hold as much shared memory
-    for (int s = 2; s <= MAX_SPLIT; s++) {
-        cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute attr[2];
-        split_config<NTOK>(cfg, attr, dim3(s, 1, 1), nullptr);
-        cfg.numAttrs = 1;
-        int n = 0;
-        HB_CUDA(cudaOccupancyMaxActiveClusters(&n, i8_split_kernel<NTOK>, &cfg));
-        g_clusters[s] = 2 * n;
-    }
     return 0;
 }
 
@@ -660,6 +650,15 @@ int i8_gemm_prepare(int sm_count) {
     if ((rc = prepare_split<16>())) return rc;
     if ((rc = prepare_split<32>())) return rc;
     if ((rc = prepare_split<64>())) return rc;
+    for (int s = 2; s <= MAX_SPLIT; s++) {  // (the tiles of 32 and 64 tokens hold as much shared memory)
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        split_config<16>(cfg, attr, dim3(s, 1, 1), nullptr);
+        cfg.numAttrs = 1;
+        int n = 0;
+        HB_CUDA(cudaOccupancyMaxActiveClusters(&n, i8_split_kernel<16>, &cfg));
+        g_clusters[s] = 2 * n;
+    }
     if ((rc = prepare_pair<128>())) return rc;
     return prepare_pair<256>();
 }

@@ -14,8 +14,10 @@
 // whose sum of squares overflows) is stored as zeros with scale NaN, so whatever is computed from it is NaN, too.
 //
 // HBM-bound: 4 B (quantize, + 4 silu_mul, + 8 add_rms_norm) read or written per element and 1 B written.  One CTA per
-// row keeps the row in registers between the reduction and the rounding (up to 32 values a thread); longer rows are
-// read twice.
+// row (a cluster of eight for a few long rows) keeps the row in registers between the reduction and the rounding, up to
+// 32 values a thread; many rows of more than 32768 columns are read twice.  Measured: quantize of 4096 x 4096 14.1 us
+// (5.9 TB/s), add_rms_norm 35 us (6.2 TB/s), silu_mul 30 us (5.0 TB/s: exp and the division take as long as the reads),
+// one row of 4096 columns 1.5 / 2.4 / 1.9 us behind its predecessor in a graph.
 //
 // Reference counterparts with a scale per 32 columns: ops::rms_norm_q8 and ops::silu_mul_q8
 // (hearth-llm/src/ops.rs:273-306, :442-504), quantize_q8_0 (hearth-quant/src/q8_0.rs:20-51).
@@ -76,50 +78,49 @@ __device__ __forceinline__ float4 mul4(float4 a, float4 b) {
     return make_float4(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y), __fmul_rn(a.z, b.z), __fmul_rn(a.w, b.w));
 }
 
-// The values v of N float4s of a row, `step` columns apart from column c (zero past the end); the norm adds h * h to `sq`
+// The values v of N float4s of a row, `step` columns apart from column c (zero past the row's end or `limit`); the norm adds h * h to `sq`
 // and writes h.  All reads of the inputs come before the first write: the compiler may not move a read over a write
 // that could be to the same memory (the sum may overwrite an input), and reads one behind the other would leave HBM idle.
 template <int OP, bool VEC, int N>
-__device__ __forceinline__ void values(const I8Rows& p, size_t row, int c, int step, float4 (&v)[N], float& sq) {
+__device__ __forceinline__ void values(const I8Rows& p, size_t row, int c, int step, int limit, float4 (&v)[N], float& sq) {
+    const int n = min(p.n_cols, limit);
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = read4<VEC>(p.x + row * p.ld, c + i * step, p.n_cols);
-    if (OP == I8_QUANTIZE) return;
-    if (OP == I8_ADD_RMS_NORM && !p.y) {
-        // h = x
-    } else {
+    for (int i = 0; i < N; i++) v[i] = read4<VEC>(p.x + row * p.ld, c + i * step, n);
+    if constexpr (OP != I8_QUANTIZE) if (OP == I8_SILU_MUL || p.y) {
         float4 y[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) y[i] = read4<VEC>(p.y + row * p.ld, c + i * step, p.n_cols);
+        for (int i = 0; i < N; i++) y[i] = read4<VEC>(p.y + row * p.ld, c + i * step, n);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (OP == I8_SILU_MUL)
+            if constexpr (OP == I8_SILU_MUL)
                 v[i] = make_float4(silu_mul1(v[i].x, y[i].x), silu_mul1(v[i].y, y[i].y), silu_mul1(v[i].z, y[i].z), silu_mul1(v[i].w, y[i].w));
             else
                 v[i] = add4(v[i], y[i]);
         }
     }
-    if (OP == I8_SILU_MUL) return;
+    if constexpr (OP == I8_ADD_RMS_NORM) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c + i * step, p.n_cols, v[i]);
-        sq = fmaf(v[i].x, v[i].x, sq);
-        sq = fmaf(v[i].y, v[i].y, sq);
-        sq = fmaf(v[i].z, v[i].z, sq);
-        sq = fmaf(v[i].w, v[i].w, sq);
+        for (int i = 0; i < N; i++) {
+            if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c + i * step, n, v[i]);
+            sq = fmaf(v[i].x, v[i].x, sq);
+            sq = fmaf(v[i].y, v[i].y, sq);
+            sq = fmaf(v[i].z, v[i].z, sq);
+            sq = fmaf(v[i].w, v[i].w, sq);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = mul4(read4<VEC>(p.weight, c + i * step, n), v[i]);
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = mul4(read4<VEC>(p.weight, c + i * step, p.n_cols), v[i]);
 }
 
 // One float4 a second time, for rows that do not fit the registers: the norm reads h back where it was written (x or r
 // may be the same memory as the sum).
 template <int OP, bool VEC>
-__device__ __forceinline__ float4 value_again(const I8Rows& p, size_t row, int c) {
+__device__ __forceinline__ float4 value_again(const I8Rows& p, size_t row, int c, int limit) {
     if (OP == I8_ADD_RMS_NORM && p.sum)
         return mul4(read4<VEC>(p.weight, c, p.n_cols), read4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols));
     float unused = 0.f;
     float4 v[1];
-    values<OP, VEC, 1>(p, row, c, 0, v, unused);
+    values<OP, VEC, 1>(p, row, c, 0, limit, v, unused);
     return v[0];
 }
 
@@ -136,14 +137,26 @@ __device__ __forceinline__ uint32_t round4(float4 v, float inv) {
                  __float2int_rn(__fmul_rn(v.w, inv)));
 }
 
-// One CTA per row.  NV = float4s of the row a thread keeps (0: the row is read twice).
-template <int OP, int NV, bool VEC, int MAX_THREADS, int MIN_CTAS>
-__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8Rows p) {
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+
+// One CTA per row, or (CLUSTER) the CTAs of a cluster, each with a run of `quads` float4s of it.  NV = float4s of the row a
+// thread keeps (0: the row is read twice).
+template <int OP, int NV, bool VEC, bool CLUSTER, int MAX_THREADS, int MIN_CTAS>
+__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8Rows p, int quads) {
     __shared__ uint32_t s_max[32];
     __shared__ float s_sq[32];
-    const int row = blockIdx.x;
+    __shared__ uint2 s_part[CLUSTER ? 8 : 1];  // maximum and sum of squares of every CTA of the row
+    const int row = CLUSTER ? blockIdx.y : blockIdx.x, rank = CLUSTER ? blockIdx.x : 0;
     const int step = blockDim.x * 4;
+    const int first = rank * quads * 4;                             // this CTA's columns: [first, padded)
+    const int padded = min((p.n_cols + 127) & ~127, first + quads * 4);
+    const int c0 = first + threadIdx.x * 4;
     pdl_trigger();
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's memory is there
     pdl_wait();
     constexpr int BATCH = NV >= 4 ? 4 : (NV > 0 ? NV : 1), BATCHES = NV > 0 ? NV / BATCH : 1;
     float4 v[BATCHES][BATCH];
@@ -151,12 +164,12 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8
     float sq = 0.f;
     if (NV > 0) {
 #pragma unroll
-        for (int b = 0; b < BATCHES; b++) values<OP, VEC, BATCH>(p, row, threadIdx.x * 4 + b * BATCH * step, step, v[b], sq);
+        for (int b = 0; b < BATCHES; b++) values<OP, VEC, BATCH>(p, row, c0 + b * BATCH * step, step, padded, v[b], sq);
 #pragma unroll
         for (int i = 0; i < NV; i++) m = absmax4(m, v[i / BATCH][i % BATCH]);
     } else {
-        for (int c = threadIdx.x * 4; c < p.n_cols; c += step) {
-            values<OP, VEC, BATCH>(p, row, c, 0, v[0], sq);
+        for (int c = c0; c < padded; c += step) {
+            values<OP, VEC, BATCH>(p, row, c, 0, padded, v[0], sq);
             m = absmax4(m, v[0][0]);
         }
     }
@@ -179,24 +192,37 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8
             for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
         }
     }
+    if (CLUSTER) {
+        const uint32_t n = gridDim.x;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (threadIdx.x < n)
+            asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(peer_smem(&s_part[rank], threadIdx.x)), "r"(m), "r"(__float_as_uint(sq)) : "memory");
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        sq = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            if (r < n) {
+                m = max(m, s_part[r].x);
+                sq += __uint_as_float(s_part[r].y);
+            }
+    }
     const float a = __uint_as_float(m);
     const bool bad = m >= 0x7F800000u || (OP == I8_ADD_RMS_NORM && !(sq <= 3.4028234e38f));
     const float inv = (!bad && a >= I8_MIN_MAX) ? __fdiv_rn(127.0f, a) : 0.0f;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && rank == 0) {
         float scale = (a >= I8_MIN_MAX) ? __fdiv_rn(a, 127.0f) : 0.0f;
         if (OP == I8_ADD_RMS_NORM) scale = __fmul_rn(scale, __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sq, (float)p.n_cols), p.eps))));
         p.scales[row] = bad ? __uint_as_float(0x7FC00000u) : scale;
     }
-    const int padded = (p.n_cols + 127) & ~127;
     if (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = threadIdx.x * 4 + i * step;
+            const int c = c0 + i * step;
             if (c < padded) *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(v[i / BATCH][i % BATCH], inv);
         }
     } else {
-        for (int c = threadIdx.x * 4; c < padded; c += step)
-            *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(value_again<OP, VEC>(p, row, c), inv);
+        for (int c = c0; c < padded; c += step)
+            *reinterpret_cast<uint32_t*>(p.plane.q + plane_off(p.plane, row, c)) = bad ? 0u : round4(value_again<OP, VEC>(p, row, c, padded), inv);
     }
 }
 
@@ -274,24 +300,34 @@ bool vec_rows(const void* p, size_t ld) { return ((reinterpret_cast<uintptr_t>(p
 
 // A launch that may start its prologue under the end of the kernel before it.
 template <typename... P, typename... A>
-int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, int cluster, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     HB_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
     return 0;
 }
 
 template <int OP, int NV, int MAX_THREADS, int MIN_CTAS>
 int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStream_t st) {
-    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, MAX_THREADS, MIN_CTAS>, dim3(n_rows),
-                      threads, st, p);
+    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, false, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, false, MAX_THREADS, MIN_CTAS>,
+                      dim3(n_rows), threads, st, 1, p, I8_MAX_COLS / 4);
+}
+template <int OP, int NV, int MAX_THREADS, int MIN_CTAS>
+int launch_rows_cluster(const I8Rows& p, int n_rows, int ctas, int quads, bool vec, cudaStream_t st) {
+    const int threads = ((quads + NV - 1) / NV + 31) / 32 * 32;
+    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, true, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, true, MAX_THREADS, MIN_CTAS>,
+                      dim3(ctas, n_rows), threads, st, ctas, p, quads);
 }
 
 template <int OP>
@@ -303,6 +339,13 @@ int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
     // Measured, us: silu_mul of 512 x 4096 4.7 with two, 7.7 with four; of 512 x 17408 20.4 with eight and two CTAs per SM,
     // 35.3 with eight and one.
     const auto resident = [&](int nv) { return threads(nv) <= 1024 && n_rows <= (long long)slot_sm_count() * (2048 / threads(nv)); };
+    // A few long rows: eight CTAs of a cluster per row (silu_mul of 32 x 17408 5.8 -> 3.3, norm of 1 x 12288 3.8 -> 2.4; from
+    // about a hundred rows on one CTA per row is ahead again, 128 x 12288 4.2 against 5.6, and so it is at 5120 columns).
+    if (quads > 1536 && n_rows <= 64) {
+        const int part = ((quads + 7) / 8 + 31) / 32 * 32;
+        if (part <= 1024) return launch_rows_cluster<OP, 1, 1024, 1>(p, n_rows, 8, part, vec, st);
+        return launch_rows_cluster<OP, 2, 1024, 1>(p, n_rows, 8, part, vec, st);
+    }
     if (resident(1)) return launch_rows_nv<OP, 1, 1024, 1>(p, n_rows, threads(1), vec, st);
     if (resident(2)) return launch_rows_nv<OP, 2, 1024, 1>(p, n_rows, threads(2), vec, st);
     if (threads(4) <= 512) return launch_rows_nv<OP, 4, 512, 2>(p, n_rows, threads(4), vec, st);
@@ -347,7 +390,7 @@ int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, 
     if (n_rows <= 0) return 0;
     const dim3 grid((n_cols + 511) / 512, (n_rows + 7) / 8);
     const bool vec = (n_cols % 4 == 0) && vec_rows(out, ld);
-    return launch_pdl(vec ? i8_dequantize_kernel<true> : i8_dequantize_kernel<false>, grid, 128, st, plane, scales, n_rows, n_cols, out, ld);
+    return launch_pdl(vec ? i8_dequantize_kernel<true> : i8_dequantize_kernel<false>, grid, 128, st, 1, plane, scales, n_rows, n_cols, out, ld);
 }
 
 }  // namespace hb200
