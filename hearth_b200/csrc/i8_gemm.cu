@@ -77,8 +77,8 @@ __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void peer_st(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ void peer_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // mbar_wait by a converged warp, whose lanes leave it together and agree on the answer.
@@ -100,16 +100,26 @@ constexpr uint32_t idesc_i8() {  // D = S32, A and B signed int8, both K-major, 
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NTOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// A CTA's share of the tokens of a tile that `split` CTAs finish together, in fours.
+__host__ __device__ constexpr int token_share(int n_tok, int split) { return ((n_tok + split - 1) / split + 3) / 4 * 4; }
+constexpr int part_bytes(int ntok) {
+    int most = 0;
+    for (int s = 2; s <= MAX_SPLIT; s++) {
+        const int b = s * 128 * token_share(ntok, s) * 4;
+        if (b > most) most = b;
+    }
+    return most;
+}
+
 template <int NTOK>
 struct SplitCfg {
     static constexpr int X_TILE = NTOK * 128;
     static constexpr int STAGE = W_TILE + X_TILE;
     // two CTAs per SM
     static constexpr int STAGES = NTOK <= 16 ? 5 : 4;
-    // Partial sums of the cluster's other CTAs: memory of their own at few tokens, else the ring's once it has run dry
-    // (`split` senders with ceil(NTOK / split) tokens of 128 rows each).
+    // Partial sums of the cluster's CTAs: memory of their own at few tokens, else the ring's once it has run dry.
     static constexpr bool OWN_PART = NTOK <= 32;
-    static constexpr int PART = (NTOK + MAX_SPLIT) * 512;
+    static constexpr int PART = part_bytes(NTOK);
     static constexpr int SMEM = STAGES * STAGE + (OWN_PART ? PART : 0) + 1024;
     static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
     static_assert(OWN_PART || PART <= STAGES * STAGE, "partial sums fit the ring");
@@ -227,57 +237,46 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
                 }
         }
     } else {
-        // Every CTA finishes its share of the tokens: the others store their sums of them into its memory, [sender][token]
-        // [128 rows] (stores do not wait for an answer; loads from the others took 6 000 cycles at 77 tokens).
-        const int share = (n_tok + split - 1) / split;
+        // Every CTA finishes its share of the tokens: all store their sums of them into its memory, [sender][four tokens]
+        // [row], 512 neighbouring bytes a warp (stores do not wait for an answer: loads from the others took 6 000 cycles at
+        // 77 tokens; single tokens a store 2 400; rows of all tokens, 16 bytes here and there, more than that).
+        const int share = token_share(n_tok, split);
         const uint32_t part = C::OWN_PART ? ring + STAGES * C::STAGE : ring;
-        const uint32_t mine = part + (uint32_t)(rank * share * 512 + (warp * 32 + lane) * 4);
+        const uint32_t mine = part + (uint32_t)(rank * share * 512 + tid * 16);
         if (!C::OWN_PART) cluster_arrive();  // this CTA's copies have landed and been read
         cluster_wait();                      // the others' memory is there (and free)
+        int owner = 0, at = 0;
         for (int c0 = 0; c0 < n_tok; c0 += 16) {
             uint32_t v[16];
             tmem_ld16(tm + c0, v);
-            int owner = c0 / share, at = c0 - owner * share;
-            uint32_t dst = peer_smem(mine, owner);
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                if (c0 + j < n_tok) peer_st(dst + at * 512, v[j]);
-                if (++at == share) { at = 0; owner++; dst = peer_smem(mine, min(owner, split - 1)); }
+            for (int j = 0; j < 16; j += 4) {
+                if (c0 + j < n_tok) peer_st4(peer_smem(mine, owner) + at * 512, v[j], v[j + 1], v[j + 2], v[j + 3]);
+                at += 4;
+                if (at == share) { at = 0; owner = min(owner + 1, split - 1); }
             }
         }
         cluster_sync();
-        const int4* sums = reinterpret_cast<const int4*>(dyn + (part - smem_u32(dyn)));
-        const int n_mine = min(share, n_tok - rank * share);
-        const bool vec = (p.ld_out % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0);
-        for (int i = tid; i < n_mine * 32; i += 128) {
+        const int first = rank * share, n_mine = min(share, n_tok - first);
+        const int4* sums = reinterpret_cast<const int4*>(dyn + (part - smem_u32(dyn))) + tid;
+        const float sw = s_sw[tid];
+        float* o = p.out + (size_t)(tok0 + first) * p.ld_out + row;
+        for (int t = 0; t < n_mine; t += 4) {
             int4 s = make_int4(0, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < MAX_SPLIT; r++)
                 if (r < split) {
-                    const int4 t = sums[r * share * 32 + i];
-                    s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+                    const int4 q = sums[(r * share + t) * 32];
+                    s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
                 }
-            const int tok = rank * share + (i >> 5), r4 = row0 + (i & 31) * 4;
-            const float sx = s_sx[tok];
-            float* o = p.out + (size_t)(tok0 + tok) * p.ld_out + r4;
-            if (!ok) continue;
-            if (vec && r4 + 3 < p.n_rows) {
-                const float4 w = *reinterpret_cast<const float4*>(&s_sw[(i & 31) * 4]);
-                float4 f = make_float4(scaled(s.x, w.x, sx), scaled(s.y, w.y, sx), scaled(s.z, w.z, sx), scaled(s.w, w.w, sx));
-                if (p.accumulate) {
-                    const float4 b = *reinterpret_cast<const float4*>(o);
-                    f = make_float4(__fadd_rn(b.x, f.x), __fadd_rn(b.y, f.y), __fadd_rn(b.z, f.z), __fadd_rn(b.w, f.w));
-                }
-                *reinterpret_cast<float4*>(o) = f;
-            } else {
-                const int q[4] = {s.x, s.y, s.z, s.w};
+            const int q[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (r4 + j < p.n_rows) {
-                        const float f = scaled(q[j], s_sw[(i & 31) * 4 + j], sx);
-                        o[j] = p.accumulate ? __fadd_rn(o[j], f) : f;
-                    }
-            }
+            for (int j = 0; j < 4; j++)
+                if (ok && row < p.n_rows && t + j < n_mine) {
+                    const float f = scaled(q[j], sw, s_sx[first + t + j]);
+                    float* d = o + (size_t)(t + j) * p.ld_out;
+                    *d = p.accumulate ? __fadd_rn(*d, f) : f;
+                }
         }
     }
     tc_fence_before();
