@@ -456,14 +456,23 @@ def matmul_f32_noalloc(w: Weight, x_dev, out_dev, ld_out: int | None = None, str
 # ---- 8-bit linear path: one scale per token, one per weight row -----------------------------------
 
 _F32 = _I8 = _raw_stream = None  # torch.float32, torch.int8 and the current stream's address of a device
+_fast = None  # the compiled checks and calls (csrc/pycall.c): a status code, or None for whatever is not the usual case
 
 
 def _i8_torch() -> None:
-    """Binds the torch names the calls below use: at one token a call's checks would otherwise cost more than its kernel."""
-    global _F32, _I8, _raw_stream
+    """Binds the torch names the calls below use, and the compiled calls: at one token a call's checks would otherwise
+    cost more than its kernel."""
+    global _F32, _I8, _raw_stream, _fast
+    if _F32 is not None:
+        return
     import torch
-    _F32, _I8 = torch.float32, torch.int8
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    from . import _pycall
+    L = _l.load()
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    hot = ("hb200_act_i8_quantize_dev", "hb200_act_i8_add_rms_norm_dev", "hb200_act_i8_silu_mul_dev", "hb200_act_i8_dequantize_dev",
+           "hb200_matmul_i8_dev")
+    _pycall.bind(torch.float32, raw_stream, *(C.cast(getattr(L, name), C.c_void_p).value for name in hot))
+    _F32, _I8, _raw_stream, _fast = torch.float32, torch.int8, raw_stream, _pycall
 
 
 def _i8_rows(name: str, t, dtype, n_cols: int, rows: int, device: int):
@@ -506,6 +515,7 @@ class WeightI8:
         r, c, d = C.c_size_t(), C.c_size_t(), C.c_int()
         check(_l.load().hb200_weight_i8_info(self._h, C.byref(r), C.byref(c), None, C.byref(d)))
         self.n_rows, self.n_cols, self.device = int(r.value), int(c.value), int(d.value)
+        self._p = self._h.value
 
     @classmethod
     def upload(cls, q: np.ndarray, scales: np.ndarray, rows: tuple[int, int] | None = None):
@@ -561,7 +571,7 @@ class WeightI8:
     def free(self) -> None:
         if self._h:
             check(_l.load().hb200_weight_i8_free(self._h))
-            self._h = None
+            self._h, self._p = None, 0
 
 
 class ActI8:
@@ -575,42 +585,49 @@ class ActI8:
         self._lib = _l.load()
         check(self._lib.hb200_act_i8_info(self._h, None, None, C.byref(d)))
         self.max_seq_len, self.n_cols, self.device = max_seq_len, n_cols, int(d.value)
+        self._p = self._h.value
 
     def _f32(self, name, t, seq_len):
         return _i8_rows(name, t, _F32, self.n_cols, seq_len, self.device)
 
     def quantize(self, x_dev, seq_len: int, stream=None) -> None:
         """Float32 rows rounded to 8 bits, a scale per row (par_quantize, hearth-llm/src/pool.rs:467, has one per 32 columns)."""
-        p, ld = self._f32("x", x_dev, seq_len)
-        rc = self._lib.hb200_act_i8_quantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
+        rc = _fast.quantize(self._p, self.device, self.n_cols, x_dev, seq_len, stream)
+        if rc is None:
+            p, ld = self._f32("x", x_dev, seq_len)
+            rc = self._lib.hb200_act_i8_quantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
         if rc:
             check(rc)
 
     def add_rms_norm(self, x_dev, weight_dev, eps: float, seq_len: int, residual_dev=None, sum_dev=None, stream=None) -> None:
         """h = x + residual (into sum_dev, which may be either of them), then weight * h / rms(h) rounded to 8 bits."""
-        p, ld = self._f32("x", x_dev, seq_len)
-        r = s = None
-        ld_s = 0
-        if residual_dev is not None:
-            r, ld_r = self._f32("residual", residual_dev, seq_len)
-            if seq_len > 1 and ld_r != ld:
-                raise Hb200Error(-4, f"x and residual have rows {ld} and {ld_r} values apart: the same distance is wanted")
-        if sum_dev is not None:
-            s, ld_s = self._f32("sum", sum_dev, seq_len)
-            if seq_len <= 1:
-                ld_s = ld
-        w = _i8_vector("weight", weight_dev, self.n_cols, self.device)
-        rc = self._lib.hb200_act_i8_add_rms_norm_dev(self._h, p, r, ld, w, eps, seq_len, s, ld_s, _i8_stream(stream, self.device))
+        rc = _fast.add_rms_norm(self._p, self.device, self.n_cols, x_dev, residual_dev, weight_dev, eps, seq_len, sum_dev, stream)
+        if rc is None:
+            p, ld = self._f32("x", x_dev, seq_len)
+            r = s = None
+            ld_s = 0
+            if residual_dev is not None:
+                r, ld_r = self._f32("residual", residual_dev, seq_len)
+                if seq_len > 1 and ld_r != ld:
+                    raise Hb200Error(-4, f"x and residual have rows {ld} and {ld_r} values apart: the same distance is wanted")
+            if sum_dev is not None:
+                s, ld_s = self._f32("sum", sum_dev, seq_len)
+                if seq_len <= 1:
+                    ld_s = ld
+            w = _i8_vector("weight", weight_dev, self.n_cols, self.device)
+            rc = self._lib.hb200_act_i8_add_rms_norm_dev(self._h, p, r, ld, w, eps, seq_len, s, ld_s, _i8_stream(stream, self.device))
         if rc:
             check(rc)
 
     def silu_mul(self, gate_dev, up_dev, seq_len: int, stream=None) -> None:
         """gate / (1 + exp(-gate)) * up rounded to 8 bits (ops::silu_mul_q8, hearth-llm/src/ops.rs:273, has a scale per 32 columns)."""
-        g, ld = self._f32("gate", gate_dev, seq_len)
-        u, ld_u = self._f32("up", up_dev, seq_len)
-        if seq_len > 1 and ld_u != ld:
-            raise Hb200Error(-4, f"gate and up have rows {ld} and {ld_u} values apart: the same distance is wanted")
-        rc = self._lib.hb200_act_i8_silu_mul_dev(self._h, g, u, ld, seq_len, _i8_stream(stream, self.device))
+        rc = _fast.silu_mul(self._p, self.device, self.n_cols, gate_dev, up_dev, seq_len, stream)
+        if rc is None:
+            g, ld = self._f32("gate", gate_dev, seq_len)
+            u, ld_u = self._f32("up", up_dev, seq_len)
+            if seq_len > 1 and ld_u != ld:
+                raise Hb200Error(-4, f"gate and up have rows {ld} and {ld_u} values apart: the same distance is wanted")
+            rc = self._lib.hb200_act_i8_silu_mul_dev(self._h, g, u, ld, seq_len, _i8_stream(stream, self.device))
         if rc:
             check(rc)
 
@@ -628,21 +645,25 @@ class ActI8:
 
     def dequantize(self, out_dev, seq_len: int, stream=None) -> None:
         """The float32 values the first seq_len rows stand for."""
-        p, ld = self._f32("out", out_dev, seq_len)
-        rc = self._lib.hb200_act_i8_dequantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
+        rc = _fast.dequantize(self._p, self.device, self.n_cols, out_dev, seq_len, stream)
+        if rc is None:
+            p, ld = self._f32("out", out_dev, seq_len)
+            rc = self._lib.hb200_act_i8_dequantize_dev(self._h, p, ld, seq_len, _i8_stream(stream, self.device))
         if rc:
             check(rc)
 
     def free(self) -> None:
         if self._h:
             check(_l.load().hb200_act_i8_free(self._h))
-            self._h = None
+            self._h, self._p = None, 0
 
 
 def matmul_i8_dev(w: WeightI8, a: ActI8, seq_len: int, out_dev, accumulate: bool = False, stream=None) -> None:
     """out[s][n] = or += sum_k(q_w q_x) * scale_w[n] * scale_x[s]; out_dev: float32 rows (strided if several products share them)."""
-    p, ld = _i8_rows("out", out_dev, _F32, w.n_rows, seq_len, w.device)
-    rc = a._lib.hb200_matmul_i8_dev(w._h, a._h, seq_len, p, ld, 1 if accumulate else 0, _i8_stream(stream, w.device))
+    rc = _fast.matmul(w._p, a._p, w.device, w.n_rows, seq_len, out_dev, accumulate, stream)
+    if rc is None:
+        p, ld = _i8_rows("out", out_dev, _F32, w.n_rows, seq_len, w.device)
+        rc = a._lib.hb200_matmul_i8_dev(w._h, a._h, seq_len, p, ld, 1 if accumulate else 0, _i8_stream(stream, w.device))
     if rc:
         check(rc)
 

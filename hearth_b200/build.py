@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -37,6 +38,21 @@ def _headers() -> list[str]:
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     hs.append(os.path.join(os.path.dirname(HERE), "include", "hb200.h"))
     return hs
+
+
+# Python's checked calls of the 8-bit linear path (pycall.c), an extension module of this interpreter.
+PYCALL = os.path.join(HERE, "_pycall.so")
+
+
+def build_pycall(force: bool = False) -> str:
+    src = os.path.join(CSRC, "pycall.c")
+    if force or _stale(PYCALL, [src]):
+        cmd = [os.environ.get("CC", "gcc"), "-O2", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"], src, "-o", PYCALL]
+        p = subprocess.run(cmd, capture_output=True, text=True)
+        if p.returncode:
+            sys.stderr.write(p.stdout + p.stderr)
+            raise RuntimeError("gcc failed on pycall.c")
+    return PYCALL
 
 
 def _stale(target: str, deps: list[str]) -> bool:
@@ -122,6 +138,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if p.returncode:
             sys.stderr.write(p.stdout + p.stderr)
             raise RuntimeError("link failed")
+    build_pycall(force)
     return LIB
 
 

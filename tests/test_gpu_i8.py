@@ -35,7 +35,7 @@ def _read(hb, act, seq):
 # ---------------------------------------------------------------------------------- rounding to 8 bits
 
 ROWS = [(1, 1), (1, 5), (2, 31), (3, 128), (7, 129), (1, 4096), (5, 4099), (9, 5120), (1, 12288), (3, 17408), (2, 32768), (2, 32772), (1, 65536), (2, 65533),
-        (300, 257), (260, 4096), (257, 8192), (256, 20000)]
+        (300, 257), (260, 4096), (257, 8192), (256, 20000), (90, 17000), (100, 12288), (65, 33000), (1000, 2050), (64, 6272)]
 
 
 @pytest.mark.parametrize("seq,cols", ROWS)

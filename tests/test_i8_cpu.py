@@ -67,3 +67,78 @@ def test_restatement_rounds_and_refuses_like_the_header_says():
     q, s = R.round_rows(big)
     assert (np.abs(q).max(axis=1) == 127).all()
     assert np.abs(q * s[:, None].astype(np.float64) - big).max() <= s.max() * (0.5 + 127 * 4 * R.U)
+
+
+class _Tensor:
+    """What the compiled checks ask of a tensor."""
+
+    def __init__(self, dtype, shape, stride, device=0, address=0x1000):
+        self.dtype, self.shape, self._stride, self._device, self._address = dtype, shape, stride, device, address
+
+    def stride(self):
+        return self._stride
+
+    def get_device(self):
+        return self._device
+
+    def data_ptr(self):
+        return self._address
+
+
+@pytest.fixture()
+def pycall(lib):
+    """The compiled calls bound to functions that record what arrives, then bound back."""
+    import torch
+    from hearth_b200 import _pycall, api
+    got = []
+    vp, sz, i, fl = C.c_void_p, C.c_size_t, C.c_int, C.c_float
+    kinds = [(vp, vp, sz, sz, vp), (vp, vp, vp, sz, vp, fl, sz, vp, sz, vp), (vp, vp, vp, sz, sz, vp), (vp, vp, sz, sz, vp), (vp, vp, sz, vp, sz, i, vp)]
+    keep = [C.CFUNCTYPE(i, *k)(lambda *a: got.append(a) or len(got)) for k in kinds]
+    _pycall.bind(torch.float32, lambda device: 0x77 + device, *(C.cast(f, vp).value for f in keep))
+    yield _pycall, got, torch
+    api._F32 = None
+    api._i8_torch()
+    del keep
+
+
+def test_compiled_calls_pass_what_they_are_given(pycall):
+    call, got, torch = pycall
+    f = torch.float32
+    x = _Tensor(f, (4, 96), (100, 1))
+    y = _Tensor(f, (5, 128), (100, 1), address=0x2000)
+    w = _Tensor(f, (96,), (1,), address=0x3000)
+    assert call.quantize(0x10, 0, 96, x, 4, None) == 1 and got[-1] == (0x10, 0x1000, 100, 4, 0x77)
+    assert call.dequantize(0x10, 0, 96, _Tensor(f, (1, 96), (1, 1)), 1, None) == 2 and got[-1] == (0x10, 0x1000, 96, 1, 0x77)
+    assert call.silu_mul(0x10, 0, 96, x, y, 4, None) == 3 and got[-1] == (0x10, 0x1000, 0x2000, 100, 4, 0x77)
+    assert call.add_rms_norm(0x10, 0, 96, x, y, w, 0.5, 4, None, None) == 4 and got[-1] == (0x10, 0x1000, 0x2000, 100, 0x3000, 0.5, 4, None, 0, 0x77)
+    assert call.add_rms_norm(0x10, 0, 96, x, None, w, 0.5, 4, y, None) == 5 and got[-1] == (0x10, 0x1000, None, 100, 0x3000, 0.5, 4, 0x2000, 100, 0x77)
+
+    class Stream:
+        cuda_stream = 0x99
+
+    assert call.matmul(0x20, 0x10, 1, 96, 4, _Tensor(f, (4, 96), (96, 1), device=1), True, Stream()) == 6
+    assert got[-1] == (0x20, 0x10, 4, 0x1000, 96, 1, 0x99)
+
+
+def test_compiled_calls_leave_everything_else_to_the_checks_in_python(pycall):
+    call, got, torch = pycall
+    f = torch.float32
+    x, w = _Tensor(f, (4, 96), (96, 1)), _Tensor(f, (96,), (1,))
+    other = [None, 3, _Tensor(torch.float16, (4, 96), (96, 1)), _Tensor(f, (4, 96), (96, 1), device=1), _Tensor(f, (4, 96), (96, 1), device=-1),
+             _Tensor(f, (3, 96), (96, 1)), _Tensor(f, (4, 95), (96, 1)), _Tensor(f, (4, 96), (1, 4)), _Tensor(f, (96,), (1,)), _Tensor(f, (1, 4, 96), (384, 96, 1))]
+    for t in other:
+        assert call.quantize(0x10, 0, 96, t, 4, None) is None
+        assert call.dequantize(0x10, 0, 96, t, 4, None) is None
+        assert call.silu_mul(0x10, 0, 96, t, x, 4, None) is None and call.silu_mul(0x10, 0, 96, x, t, 4, None) is None
+        assert call.add_rms_norm(0x10, 0, 96, t, None, w, 0.5, 4, None, None) is None
+        assert call.matmul(0x20, 0x10, 0, 96, 4, t, False, None) is None
+        if t is not None:
+            assert call.add_rms_norm(0x10, 0, 96, x, t, w, 0.5, 4, None, None) is None
+            assert call.add_rms_norm(0x10, 0, 96, x, None, w, 0.5, 4, t, None) is None
+    wide = _Tensor(f, (4, 96), (97, 1))
+    assert call.silu_mul(0x10, 0, 96, x, wide, 4, None) is None and call.add_rms_norm(0x10, 0, 96, x, wide, w, 0.5, 4, None, None) is None
+    assert call.add_rms_norm(0x10, 0, 96, x, None, x, 0.5, 4, None, None) is None and call.add_rms_norm(0x10, 0, 96, x, None, w, 1, 4, None, None) is None
+    assert call.quantize(0x10, 0, 96, x, -1, None) is None and call.quantize(0x10, 0, 96, x, 4, "stream") is None and call.quantize(0x10, 0, 96, x) is None
+    assert not got
+    with pytest.raises(TypeError):
+        call.bind(f, None, 0, 0, 0, 0, 0)
