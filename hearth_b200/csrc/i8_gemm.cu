@@ -92,6 +92,11 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return false;
 }
 
+// The last commit of a CTA, awaited with a limit whether or not the CTA is giving up.
+__device__ __forceinline__ void await_mmas(uint32_t bar) {
+    for (uint32_t i = 0; i < SPIN_LIMIT && !__all_sync(0xffffffffu, mbar_try(bar, 0)); i++) {}
+}
+
 // The order of the two multiplications keeps an intermediate of tiny scales out of the subnormals.
 __device__ __forceinline__ float scaled(int acc, float sw, float sx) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), sw), sx); }
 
@@ -205,11 +210,17 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) mma_i8(tmem, ad + 2 * j, bd + 2 * j, idesc_i8<NTOK>(), (i | j) != 0);
                 tc_commit(smem_u32(&empty[s]));
-                if (i == nk - 1) tc_commit(smem_u32(&done));
             }
             __syncwarp();
         }
-        if (!mbar_wait_warp(smem_u32(&done), 0, &abort_flag, p.status, 62)) failed = 1;
+        // also after a wait that ran out: no MMA may still read this CTA's memory when it ends
+        if (elect_one()) tc_commit(smem_u32(&done));
+        __syncwarp();
+        await_mmas(smem_u32(&done));
+        if (*(volatile int*)&abort_flag || !mbar_try(smem_u32(&done), 0)) {
+            atomicCAS(p.status, 0, 62);
+            failed = 1;
+        }
         __syncwarp();
     } else if (warp == 2) {
         for (int t = lane; t < NTOK; t += 32) s_sx[t] = t < n_tok ? p.sx[tok0 + t] : 0.f;
@@ -379,8 +390,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     constexpr int STAGES = C::STAGES;
     extern __shared__ unsigned char dyn[];
     // full: this CTA's copies of a stage; peer_full (leader): the other CTA's; empty: the stage may be refilled;
-    // acc_full / acc_empty: an accumulator is complete / has been read (leader: by both CTAs' epilogue warps)
-    __shared__ uint64_t full[STAGES], peer_full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+    // acc_full / acc_empty: an accumulator is complete / has been read (leader: by both CTAs' epilogue warps); drained: no
+    // MMA is under way any more
+    __shared__ uint64_t full[STAGES], peer_full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -414,6 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
             mbar_init(smem_u32(&acc_full[a]), 1);
             mbar_init(smem_u32(&acc_empty[a]), 2 * PAIR_EPI_WARPS);
         }
+        mbar_init(smem_u32(&drained), 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (int k = 0; k < ahead; k++) {
@@ -508,7 +521,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
                 if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
+        // also after a wait that ran out: no MMA may still read either CTA's memory when they end
+        if (rank == 0 && elect_one()) commit_pair(smem_u32(&drained));
         __syncwarp();
+        await_mmas(smem_u32(&drained));
     } else {
         const int q = warp & 3;                      // TMEM lane quarter of this warp
         const int half = (warp - 2) / 4 * (NT / 2);  // its first token of the tile

@@ -232,7 +232,8 @@ def test_silu_mul_extremes(hb):
 
 PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 4096, 300), (2, 129, 127), (8, 64, 1), (15, 100, 257), (16, 2048, 256), (17, 640, 130), (31, 1, 129),
             (32, 5120, 512), (33, 300, 64), (64, 1152, 384), (65, 1000, 200), (77, 2050, 1024), (128, 512, 128), (129, 2048, 384), (200, 4097, 129),
-            (256, 256, 256), (257, 384, 300), (300, 1111, 777), (513, 384, 700), (1000, 896, 515), (1024, 1024, 2048), (2049, 130, 1025)]
+            (256, 256, 256), (257, 384, 300), (300, 1111, 777), (513, 384, 700), (1000, 896, 515), (1024, 1024, 2048), (2049, 130, 1025),
+            (2600, 1411, 2100), (2333, 2049, 2900), (1025, 3333, 2700), (5003, 1665, 1153)]
 
 
 def _product_case(hb, seq, cols, rows, key=0):
@@ -569,3 +570,126 @@ def test_objects_of_two_slots(hb):
             h.free()
     finally:
         hb.set_slot(0)
+
+
+# ---------------------------------------------------------------------------------- order, graphs, far offsets
+
+def test_captured_behind_copies_and_beside_another_stream(hb):
+    """A graph whose calls follow a copy node and join a forked stream: the early start of the kernels must not outrun
+    either."""
+    import torch
+    cols, rows, seq = 1536, 520, 30
+    W = hb.WeightI8.quantize_dev(_cuda(_rng(41).standard_normal((rows, cols)).astype(np.float32)))
+    A, B = hb.ActI8(seq, cols), hb.ActI8(seq, cols)
+    src = [torch.randn(seq, cols, device="cuda") for _ in range(6)]
+    xa, xb = torch.zeros(seq, cols, device="cuda"), torch.zeros(seq, cols, device="cuda")
+    oa, ob = torch.zeros(seq, rows, device="cuda"), torch.zeros(seq, rows, device="cuda")
+    pick = torch.zeros(seq, cols, device="cuda")
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        xa.copy_(pick)                       # a copy node in front of the first call
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            torch.mul(pick, 2.0, out=xb)
+            B.quantize(xb, seq)
+            hb.matmul_i8_dev(W, B, seq, ob)
+        A.quantize(xa, seq)
+        hb.matmul_i8_dev(W, A, seq, oa)
+        main.wait_stream(side)
+        oa.add_(ob)
+        A.quantize(xa, seq)
+        hb.matmul_i8_dev(W, A, seq, oa, accumulate=True)
+
+    side, st = torch.cuda.Stream(), torch.cuda.Stream()
+    want = []
+    for s in src:
+        pick.copy_(s)
+        torch.cuda.synchronize()
+        step(side)
+        torch.cuda.synchronize()
+        want.append(oa.clone())
+    g = torch.cuda.CUDAGraph()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=st):
+        step(side)
+    for _ in range(3):
+        for s, e in zip(src, want):
+            pick.copy_(s)
+            g.replay()
+            assert torch.equal(oa, e)
+    for h in (W, A, B):
+        h.free()
+
+
+def test_two_graphs_of_the_same_weight(hb):
+    """Two captured products of one weight, replayed on two streams at once: a call keeps no scratch."""
+    import torch
+    cols, rows = 4096, 1024
+    W = hb.WeightI8.quantize_dev(torch.randn(rows, cols, device="cuda"))
+    parts = []
+    for seq in (1, 40):
+        A, x, out = hb.ActI8(seq, cols), torch.randn(seq, cols, device="cuda"), torch.empty(seq, rows, device="cuda")
+        A.quantize(x, seq)
+        hb.matmul_i8_dev(W, A, seq, out)
+        want, st, g = out.clone(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=st):
+            for _ in range(20):
+                A.quantize(x, seq)
+                hb.matmul_i8_dev(W, A, seq, out)
+        parts.append((A, out, want, st, g))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _, out, _, st, g in parts:
+            with torch.cuda.stream(st):
+                out.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    for A, out, want, _, _ in parts:
+        assert torch.equal(out, want)
+        A.free()
+    W.free()
+
+
+def test_offsets_past_32_bits(hb):
+    """An activation plane of 2.1 GB, inputs and outputs of more than 2^31 values: the last tokens come out right."""
+    import torch
+    seq, cols, rows = 65535, 33000, 150
+    x = torch.zeros(seq, cols, device="cuda")
+    tail = _rng(61).standard_normal((7, cols)).astype(np.float32)
+    x[-7:] = _cuda(tail)
+    A = hb.ActI8(seq, cols)
+    A.quantize(x, seq)
+    q, s = R.round_rows(tail)
+    qw = _ints(_rng(62), rows, cols)
+    sw = np.full(rows, 1e-3, dtype=np.float32)
+    W = hb.WeightI8.upload(qw, sw)
+    out = torch.empty(seq, rows, device="cuda")
+    hb.matmul_i8_dev(W, A, seq, out)
+    want = R.product(qw, sw, q, s)
+    assert (np.abs(out[-7:].cpu().numpy() - want) <= R.PRODUCT_RTOL * np.abs(want)).all() and not out[:-7].any()
+    A.dequantize(x, seq)
+    assert np.array_equal(x[-7:].cpu().numpy(), q.astype(np.float32) * s[:, None])
+    A.free(); W.free()
+    del x, out
+    rows, cols = 40000, 64
+    qw, qx = _ints(_rng(63), rows, cols), _ints(_rng(64), 3, cols)
+    W = hb.WeightI8.upload(qw, np.ones(rows, dtype=np.float32))
+    A = hb.ActI8(seq, cols)
+    A.load(torch.zeros(seq, cols, dtype=torch.int8, device="cuda"), torch.ones(seq, device="cuda"), seq)
+    rows_q = torch.zeros(seq, cols, dtype=torch.int8, device="cuda")
+    rows_q[-3:] = _cuda(qx)
+    A.load(rows_q, torch.ones(seq, device="cuda"), seq)
+    out = torch.empty(seq, rows, device="cuda")
+    hb.matmul_i8_dev(W, A, seq, out)
+    assert np.array_equal(out[-3:].cpu().numpy(), (qx.astype(np.int64) @ qw.astype(np.int64).T).astype(np.float32))
+    assert not out[-10000:-3].any()
+    hb.check_status()
+    A.free(); W.free()
+
+
+def test_every_kernel_variant_is_covered_by_a_shape_above(hb):
+    names = {hb.matmul_i8_kernel(n, k, m) for m, k, n in PRODUCTS}
+    assert names == {"i8_tcgen05_n16", "i8_tcgen05_n16_split", "i8_tcgen05_n32", "i8_tcgen05_n32_split", "i8_tcgen05_n64", "i8_tcgen05_n64_split",
+                     "i8_tcgen05_pair_n128", "i8_tcgen05_pair_n256"}, names
