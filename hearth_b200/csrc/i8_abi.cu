@@ -3,7 +3,7 @@
 // i8_gemm.cu.  Errors never cross the boundary as exceptions.
 #include <cuda.h>
 
-#include <map>
+#include <cfloat>
 #include <new>
 
 #include "../../include/hb200.h"
@@ -397,7 +397,7 @@ extern "C" int hb200_act_i8_add_rms_norm_dev(hb200_act_i8_t a, const float* x_de
     if ((rc = check_seq(a, seq_len))) return rc;
     if ((rc = check_ld("ld_x", ld_x, a->n_cols))) return rc;
     if (sum_dev && (rc = check_ld("ld_sum", ld_sum, a->n_cols))) return rc;
-    if (!(eps > 0.0f) || eps > 3.0e38f) { set_error("eps %g: a positive finite number", (double)eps); return HB200_ERR_BAD_SHAPE; }
+    if (!(eps > 0.0f && eps <= FLT_MAX)) { set_error("eps %g: a positive finite number", (double)eps); return HB200_ERR_BAD_SHAPE; }
     if (sum_dev && ld_sum != ld_x && (sum_dev == x_dev || sum_dev == residual_dev)) {
         set_error("the sum overwrites an input row by row: ld_sum %zu must be ld_x %zu", ld_sum, ld_x);
         return HB200_ERR_BAD_SHAPE;

@@ -2,7 +2,8 @@
  * checks in Python, two such calls cost more host time (about 4 us) than their kernels run; here the checks of the usual
  * case - two-dimensional CUDA tensors of the right type on the handle's device - and the call itself take a tenth of it.
  * Anything else (another shape, type or device, a missing tensor) returns None, and api.py's own checks then refuse or
- * serve it; a number is the call's status code.  The C entry points are those of the library that ctypes loaded. */
+ * serve it; a number is the call's status code.  The C entry points are those of the library that ctypes loaded; like
+ * ctypes, the calls let other Python threads run meanwhile (a full launch queue blocks). */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stddef.h>
@@ -100,7 +101,11 @@ static PyObject *quantize(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     if (n != 6 || !number(a[0], &h) || !number(a[1], &dev) || !number(a[2], &cols) || !number(a[4], &seq) ||
         !rows_of(a[3], cols, seq, dev, &x, &ld) || !stream_of(a[5], a[1], &st))
         Py_RETURN_NONE;
-    return PyLong_FromLong(f_quantize((void *)h, x, ld, seq, st));
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_quantize((void *)h, x, ld, seq, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
 }
 
 /* add_rms_norm(act, device, n_cols, x, residual or None, weight, eps, seq_len, sum or None, stream) */
@@ -115,7 +120,12 @@ static PyObject *add_rms_norm(PyObject *self, PyObject *const *a, Py_ssize_t n) 
     if (a[8] != Py_None && !rows_of(a[8], cols, seq, dev, &s, &ld_s)) Py_RETURN_NONE;
     if (!stream_of(a[9], a[1], &st)) Py_RETURN_NONE;
     if (s && seq <= 1) ld_s = ld;
-    return PyLong_FromLong(f_norm((void *)h, x, r, ld, w, (float)PyFloat_AS_DOUBLE(a[6]), seq, s, ld_s, st));
+    const float eps = (float)PyFloat_AS_DOUBLE(a[6]);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_norm((void *)h, x, r, ld, w, eps, seq, s, ld_s, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
 }
 
 /* silu_mul(act, device, n_cols, gate, up, seq_len, stream) */
@@ -127,7 +137,11 @@ static PyObject *silu_mul(PyObject *self, PyObject *const *a, Py_ssize_t n) {
         !rows_of(a[3], cols, seq, dev, &g, &ld) || !rows_of(a[4], cols, seq, dev, &u, &ld_u) || (ld_u != ld && seq > 1) ||
         !stream_of(a[6], a[1], &st))
         Py_RETURN_NONE;
-    return PyLong_FromLong(f_silu((void *)h, g, u, ld, seq, st));
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_silu((void *)h, g, u, ld, seq, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
 }
 
 /* dequantize(act, device, n_cols, out, seq_len, stream) */
@@ -138,7 +152,11 @@ static PyObject *dequantize(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     if (n != 6 || !number(a[0], &h) || !number(a[1], &dev) || !number(a[2], &cols) || !number(a[4], &seq) ||
         !rows_of(a[3], cols, seq, dev, &o, &ld) || !stream_of(a[5], a[1], &st))
         Py_RETURN_NONE;
-    return PyLong_FromLong(f_dequantize((void *)h, o, ld, seq, st));
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_dequantize((void *)h, o, ld, seq, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
 }
 
 /* matmul(weight, act, device, n_rows, seq_len, out, accumulate, stream) */
@@ -151,7 +169,11 @@ static PyObject *matmul(PyObject *self, PyObject *const *a, Py_ssize_t n) {
         Py_RETURN_NONE;
     const int acc = PyObject_IsTrue(a[6]);
     if (acc < 0) { PyErr_Clear(); Py_RETURN_NONE; }
-    return PyLong_FromLong(f_matmul((void *)w, (void *)h, seq, o, ld, acc, st));
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_matmul((void *)w, (void *)h, seq, o, ld, acc, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
 }
 
 /* bind(torch.float32, raw_stream, addresses of quantize, add_rms_norm, silu_mul, dequantize, matmul) */
