@@ -510,7 +510,6 @@ class WeightI8:
     """An int8 weight matrix with one f32 scale per row (output channel), resident on the device."""
 
     def __init__(self, handle):
-        _i8_torch()
         self._h = handle
         r, c, d = C.c_size_t(), C.c_size_t(), C.c_int()
         check(_l.load().hb200_weight_i8_info(self._h, C.byref(r), C.byref(c), None, C.byref(d)))
@@ -558,6 +557,7 @@ class WeightI8:
 
     def store(self, q_dev=None, scales_dev=None, stream=None) -> None:
         """Row-major values and scales back into CUDA tensors (either may be None)."""
+        _i8_torch()
         p, ld = _i8_rows("values", q_dev, _I8, self.n_cols, self.n_rows, self.device) if q_dev is not None else (None, 0)
         s = _i8_vector("scales", scales_dev, self.n_rows, self.device) if scales_dev is not None else None
         check(_l.load().hb200_weight_i8_store_dev(self._h, p, ld, s, _i8_stream(stream, self.device)))

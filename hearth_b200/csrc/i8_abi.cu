@@ -124,27 +124,25 @@ int weight_new(size_t n_rows, size_t n_cols, hb200_weight_i8** out) {
     const size_t tiles = (n_rows + 127) / 128, bytes = tiles * w->plane.tile_stride, sbytes = tiles * 128 * sizeof(float);
     w->resident_bytes = bytes + sbytes;
     if (tiles > 0) {
-        cudaError_t e = cudaMalloc(&w->plane.q, bytes);
-        if (e == cudaSuccess) e = cudaMalloc(&w->scales, sbytes);
+        cudaError_t e = cudaMalloc(&w->plane.q, bytes + sbytes);  // the scales behind the plane
         // rows past the last one take part in the product of their tile (and are not stored)
-        if (e == cudaSuccess) e = cudaMemset(w->plane.q + (tiles - 1) * w->plane.tile_stride, 0, w->plane.tile_stride);
-        if (e == cudaSuccess) e = cudaMemset(w->scales, 0, sbytes);
+        const size_t keep = (tiles - 1) * w->plane.tile_stride;
+        if (e == cudaSuccess) e = cudaMemset(w->plane.q + keep, 0, bytes - keep + sbytes);
         if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
         if (e != cudaSuccess) {
             set_error("weight of %zu x %zu: %s", n_rows, n_cols, cudaGetErrorString(e));
             cudaGetLastError();
             if (w->plane.q) cudaFree(w->plane.q);
-            if (w->scales) cudaFree(w->scales);
             delete w;
             return HB200_ERR_CUDA;
         }
+        w->scales = reinterpret_cast<float*>(w->plane.q + bytes);
     }
     *out = w;
     return 0;
 }
 void weight_delete(hb200_weight_i8* w) {
     if (w->plane.q) cudaFree(w->plane.q);
-    if (w->scales) cudaFree(w->scales);
     delete w;
 }
 // The weight is complete when the call returns: the product reads it ahead of its stream's order.
@@ -334,19 +332,17 @@ extern "C" int hb200_act_i8_create(size_t max_seq_len, size_t n_cols, hb200_act_
     a->plane.kb_stride = groups * 1024;
     a->plane.row_shift = 3;
     const size_t bytes = (size_t)a->kb * a->plane.kb_stride, sbytes = groups * 8 * sizeof(float);
-    cudaError_t e = cudaMalloc(&a->plane.q, bytes);
-    if (e == cudaSuccess) e = cudaMalloc(&a->scales, sbytes);
-    if (e == cudaSuccess) e = cudaMemset(a->plane.q, 0, bytes);
-    if (e == cudaSuccess) e = cudaMemset(a->scales, 0, sbytes);
+    cudaError_t e = cudaMalloc(&a->plane.q, bytes + sbytes);  // the scales behind the plane
+    if (e == cudaSuccess) e = cudaMemset(a->plane.q, 0, bytes + sbytes);
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
         set_error("activation allocation failed: %s", cudaGetErrorString(e));
         cudaGetLastError();
         if (a->plane.q) cudaFree(a->plane.q);
-        if (a->scales) cudaFree(a->scales);
         delete a;
         return HB200_ERR_CUDA;
     }
+    a->scales = reinterpret_cast<float*>(a->plane.q + bytes);
     *out = a;
     return HB200_OK;
     I8_END
@@ -357,7 +353,6 @@ extern "C" int hb200_act_i8_free(hb200_act_i8_t a) {
     if (!a) return HB200_OK;
     I8_USE(a->slot);
     if (a->plane.q) cudaFree(a->plane.q);
-    if (a->scales) cudaFree(a->scales);
     delete a;
     return HB200_OK;
     I8_END
@@ -537,7 +532,6 @@ void i8_release_slot(int slot) {
     if (g.out) cudaFree(g.out);
     if (g.act) {
         if (g.act->plane.q) cudaFree(g.act->plane.q);
-        if (g.act->scales) cudaFree(g.act->scales);
         delete g.act;
     }
     g = Staging();

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
             bulk_load(ring + i * C::STAGE, wp + (size_t)i * W_TILE, W_TILE, smem_u32(&full[i]));
         }
     }
+    __syncwarp();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
                     const float r = scaled((int)v[j], sw, s_sx[c0 + j]);
                     *o = p.accumulate ? __fadd_rn(*o, r) : r;
                 }
+            __syncwarp();  // the lanes of rows past the end rejoin before the next TMEM load
         }
     } else {
         // Every CTA finishes its share of the tokens: all store their sums of them into its memory, [sender][four tokens]
@@ -444,6 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
             bulk_load(ring + k * C::STAGE, w_src(t0) + (size_t)k * 2 * W_TILE, blocks * W_TILE, full0 + k * 8);
         }
     }
+    __syncwarp();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -561,6 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
                 } else {
                     store_cols<ACC, true>(o, p.ld_out, v, sw, sx, live, n_tok - c0);
                 }
+                __syncwarp();  // the lanes of rows past the end rejoin before the next TMEM load
             }
             tc_fence_before();
             __syncwarp();
@@ -568,6 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         }
         __syncwarp();
     }
+    __syncwarp();
     tc_fence_before();
     cluster_sync();  // the other CTA may still read this one's operands or signal its barriers
     if (warp == 1) {

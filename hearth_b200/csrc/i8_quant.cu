@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (threadIdx.x < n)
             asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(peer_smem(&s_part[rank], threadIdx.x)), "r"(m), "r"(__float_as_uint(sq)) : "memory");
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         sq = 0.f;
 #pragma unroll
@@ -226,47 +227,70 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8
     }
 }
 
-// Row-major int8 rows (`ld` bytes apart) -> plane; columns past n_cols become zero.  grid (columns / 512, rows).
+// Row-major int8 rows (`ld` bytes apart) <-> plane, a 16-byte piece of four rows a thread.  grid (columns / 2048, rows / 4 at
+// most 65535).
+constexpr int MOVE_ROWS = 4;
+
+// -> plane; columns past n_cols become zero.
 __global__ void __launch_bounds__(128) i8_load_kernel(const int8_t* q, size_t ld, const float* scales_in, int n_rows, int n_cols, I8Plane plane,
                                                       float* scales) {
     pdl_trigger();
     pdl_wait();
-    const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
-    const int padded = (n_cols + 127) & ~127;
-    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
-        if (c < padded) {
-            const int8_t* src = q + (size_t)row * ld;
-            uint32_t v = 0;
-            if (c + 3 < n_cols && ((reinterpret_cast<uintptr_t>(src + c) & 3) == 0)) {
-                v = *reinterpret_cast<const uint32_t*>(src + c);
+    const int c = (blockIdx.x * 128 + threadIdx.x) * 16;
+    if (c >= ((n_cols + 127) & ~127)) return;
+    const bool whole = c + 16 <= n_cols && ((reinterpret_cast<uintptr_t>(q) | ld) & 15) == 0;
+    for (size_t row0 = (size_t)blockIdx.y * MOVE_ROWS; row0 < (size_t)n_rows; row0 += (size_t)gridDim.y * MOVE_ROWS) {
+        uint4 v[MOVE_ROWS];
+#pragma unroll
+        for (int i = 0; i < MOVE_ROWS; i++) {
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (row0 + i >= (size_t)n_rows) continue;
+            const int8_t* src = q + (row0 + i) * ld + c;
+            if (whole) {
+                v[i] = *reinterpret_cast<const uint4*>(src);
             } else {
-                for (int i = 0; i < 4; i++)
-                    if (c + i < n_cols) v |= (uint32_t)(uint8_t)src[c + i] << (8 * i);
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (c + j < n_cols) w[j / 4] |= (uint32_t)(uint8_t)src[j] << (8 * (j % 4));
+                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            *reinterpret_cast<uint32_t*>(plane.q + plane_off(plane, row, c)) = v;
         }
-        if (c == 0) scales[row] = scales_in[row];
+#pragma unroll
+        for (int i = 0; i < MOVE_ROWS; i++) {
+            if (row0 + i >= (size_t)n_rows) continue;
+            *reinterpret_cast<uint4*>(plane.q + plane_off(plane, (int)row0 + i, c)) = v[i];
+            if (c == 0) scales[row0 + i] = scales_in[row0 + i];
+        }
     }
 }
 
-// Plane -> row-major int8 rows and / or scales.
+// Plane -> row-major rows and / or scales.
 __global__ void __launch_bounds__(128) i8_store_kernel(I8Plane plane, const float* scales, int n_rows, int n_cols, int8_t* q, size_t ld,
                                                        float* scales_out) {
     pdl_trigger();
     pdl_wait();
-    const int c = (blockIdx.x * 128 + threadIdx.x) * 4;
-    for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
-        if (q && c < n_cols) {
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(plane.q + plane_off(plane, row, c));
-            int8_t* dst = q + (size_t)row * ld + c;
-            if (c + 3 < n_cols && ((reinterpret_cast<uintptr_t>(dst) & 3) == 0)) {
-                *reinterpret_cast<uint32_t*>(dst) = v;
-            } else {
-                for (int i = 0; i < 4; i++)
-                    if (c + i < n_cols) dst[i] = (int8_t)(v >> (8 * i));
+    const int c = (blockIdx.x * 128 + threadIdx.x) * 16;
+    if (c >= n_cols) return;
+    const bool whole = c + 16 <= n_cols && ((reinterpret_cast<uintptr_t>(q) | ld) & 15) == 0;
+    for (size_t row0 = (size_t)blockIdx.y * MOVE_ROWS; row0 < (size_t)n_rows; row0 += (size_t)gridDim.y * MOVE_ROWS) {
+#pragma unroll
+        for (int i = 0; i < MOVE_ROWS; i++) {
+            if (row0 + i >= (size_t)n_rows) continue;
+            if (q) {
+                const uint4 v = *reinterpret_cast<const uint4*>(plane.q + plane_off(plane, (int)row0 + i, c));
+                int8_t* dst = q + (row0 + i) * ld + c;
+                if (whole) {
+                    *reinterpret_cast<uint4*>(dst) = v;
+                } else {
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (c + j < n_cols) dst[j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
+                }
             }
+            if (scales_out && c == 0) scales_out[row0 + i] = scales[row0 + i];
         }
-        if (scales_out && c == 0) scales_out[row] = scales[row];
     }
 }
 
@@ -355,7 +379,10 @@ int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
     return launch_rows_nv<OP, 0, 1024, 1>(p, n_rows, 1024, vec, st);
 }
 
-dim3 move_grid(int n_rows, int n_cols) { return dim3((((n_cols + 127) & ~127) + 511) / 512, n_rows < 65535 ? n_rows : 65535); }
+dim3 move_grid(int n_rows, int n_cols) {
+    const int rows = (n_rows + MOVE_ROWS - 1) / MOVE_ROWS;
+    return dim3((n_cols + 2047) / 2048, rows < 65535 ? rows : 65535);
+}
 
 }  // namespace
 
@@ -374,16 +401,12 @@ int launch_i8_rows(int op, const I8Rows& p, int n_rows, cudaStream_t st) {
 
 int launch_i8_load(const int8_t* q, size_t ld, const float* scales_in, int n_rows, int n_cols, const I8Plane& plane, float* scales, cudaStream_t st) {
     if (n_rows <= 0) return 0;
-    i8_load_kernel<<<move_grid(n_rows, n_cols), 128, 0, st>>>(q, ld, scales_in, n_rows, n_cols, plane, scales);
-    HB_CUDA(cudaGetLastError());
-    return 0;
+    return launch_pdl(i8_load_kernel, move_grid(n_rows, n_cols), 128, st, 1, q, ld, scales_in, n_rows, n_cols, plane, scales);
 }
 
 int launch_i8_store(const I8Plane& plane, const float* scales, int n_rows, int n_cols, int8_t* q, size_t ld, float* scales_out, cudaStream_t st) {
     if (n_rows <= 0) return 0;
-    i8_store_kernel<<<move_grid(n_rows, n_cols), 128, 0, st>>>(plane, scales, n_rows, n_cols, q, ld, scales_out);
-    HB_CUDA(cudaGetLastError());
-    return 0;
+    return launch_pdl(i8_store_kernel, move_grid(n_rows, n_cols), 128, st, 1, plane, scales, n_rows, n_cols, q, ld, scales_out);
 }
 
 int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld, cudaStream_t st) {

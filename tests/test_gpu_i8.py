@@ -111,26 +111,29 @@ def test_rows_behind_the_last_are_left(hb):
     A.dequantize(v, 3)
     assert (v[3:] == 5).all()
     A.quantize(_cuda(x), 0)  # nothing to do
+    A.quantize(_cuda(y[0]), 1)  # one row as a vector
     assert np.array_equal(_read(hb, A, 20)[0], want_q)
     A.free()
 
 
-@pytest.mark.parametrize("ld", [77, 80])
-def test_load_and_store_round_trip(hb, ld):
+@pytest.mark.parametrize("rows,cols,ld,shift", [(11, 77, 77, 0), (11, 77, 80, 0), (5, 128, 128, 1), (3, 2048, 2064, 0), (6, 2100, 2112, 16), (1, 4097, 4100, 0),
+                                                (9, 16, 16, 0), (2, 1, 1, 3)])
+def test_load_and_store_round_trip(hb, rows, cols, ld, shift):
     import torch
-    q = _ints(_rng(ld), 11, 77)
-    s = _rng(ld, 2).random(11).astype(np.float32)
-    buf = torch.zeros(11, ld, dtype=torch.int8, device="cuda")
-    buf[:, :77] = _cuda(q)
-    A = hb.ActI8(16, 77)
-    A.load(buf[:, :77], _cuda(s), 11)
-    got_q, got_s = _read(hb, A, 11)
+    q = _ints(_rng(ld, rows), rows, cols)
+    s = _rng(ld, 2).random(rows).astype(np.float32)
+    buf = torch.zeros(rows * ld + shift, dtype=torch.int8, device="cuda")[shift:].view(rows, ld)
+    buf[:, :cols] = _cuda(q)
+    A = hb.ActI8(16, cols)
+    A.load(buf[:, :cols], _cuda(s), rows)
+    got_q, got_s = _read(hb, A, rows)
     assert np.array_equal(got_q, q) and np.array_equal(got_s, s)
-    back = torch.full((11, ld), 3, dtype=torch.int8, device="cuda")
-    A.store(back[:, :77], None, 11)
-    assert np.array_equal(back[:, :77].cpu().numpy(), q) and (back[:, 77:] == 3).all()
-    only = torch.zeros(11, device="cuda")
-    A.store(None, only, 11)
+    flat = torch.full((rows * ld + shift,), 3, dtype=torch.int8, device="cuda")
+    back = flat[shift:].view(rows, ld)
+    A.store(back[:, :cols], None, rows)
+    assert np.array_equal(back[:, :cols].cpu().numpy(), q) and (back[:, cols:] == 3).all() and (flat[:shift] == 3).all()
+    only = torch.zeros(rows, device="cuda")
+    A.store(None, only, rows)
     assert np.array_equal(only.cpu().numpy(), s)
     A.free()
 
