@@ -456,7 +456,7 @@ def matmul_f32_noalloc(w: Weight, x_dev, out_dev, ld_out: int | None = None, str
 # ---- 8-bit linear path: one scale per token, one per weight row -----------------------------------
 
 _F32 = _I8 = _raw_stream = None  # torch.float32, torch.int8 and the current stream's address of a device
-_fast = None  # the compiled checks and calls (csrc/pycall.c): a status code, or None for whatever is not the usual case
+_fast = None  # the compiled checks and calls (csrc/pycall.cpp): a status code, or None for whatever is not the usual case
 
 
 def _i8_torch() -> None:
@@ -471,7 +471,7 @@ def _i8_torch() -> None:
     raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
     hot = ("hb200_act_i8_quantize_dev", "hb200_act_i8_add_rms_norm_dev", "hb200_act_i8_silu_mul_dev", "hb200_act_i8_dequantize_dev",
            "hb200_matmul_i8_dev")
-    _pycall.bind(torch.float32, raw_stream, *(C.cast(getattr(L, name), C.c_void_p).value for name in hot))
+    _pycall.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in hot))
     _F32, _I8, _raw_stream, _fast = torch.float32, torch.int8, raw_stream, _pycall
 
 

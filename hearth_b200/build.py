@@ -40,18 +40,24 @@ def _headers() -> list[str]:
     return hs
 
 
-# Python's checked calls of the 8-bit linear path (pycall.c), an extension module of this interpreter.
+# Python's checked calls of the 8-bit linear path (pycall.cpp), an extension module of this interpreter and its torch.
 PYCALL = os.path.join(HERE, "_pycall.so")
 
 
 def build_pycall(force: bool = False) -> str:
-    src = os.path.join(CSRC, "pycall.c")
+    src = os.path.join(CSRC, "pycall.cpp")
     if force or _stale(PYCALL, [src]):
-        cmd = [os.environ.get("CC", "gcc"), "-O2", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"], src, "-o", PYCALL]
+        import torch
+        root = os.path.dirname(torch.__file__)
+        cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
+        include = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                   os.path.join(cuda, "include")]
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+        cmd += [f"-I{d}" for d in include] + [src, "-o", PYCALL, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
         p = subprocess.run(cmd, capture_output=True, text=True)
         if p.returncode:
             sys.stderr.write(p.stdout + p.stderr)
-            raise RuntimeError("gcc failed on pycall.c")
+            raise RuntimeError("g++ failed on pycall.cpp")
     return PYCALL
 
 

@@ -69,76 +69,66 @@ def test_restatement_rounds_and_refuses_like_the_header_says():
     assert np.abs(q * s[:, None].astype(np.float64) - big).max() <= s.max() * (0.5 + 127 * 4 * R.U)
 
 
-class _Tensor:
-    """What the compiled checks ask of a tensor."""
-
-    def __init__(self, dtype, shape, stride, device=0, address=0x1000):
-        self.dtype, self.shape, self._stride, self._device, self._address = dtype, shape, stride, device, address
-
-    def stride(self):
-        return self._stride
-
-    def get_device(self):
-        return self._device
-
-    def data_ptr(self):
-        return self._address
-
-
 @pytest.fixture()
 def pycall(lib):
-    """The compiled calls bound to functions that record what arrives, then bound back."""
+    """The compiled calls bound to functions that record what arrives, then bound back.  Device -1 stands for the CPU."""
     import torch
-    from hearth_b200 import _pycall, api
+    from hearth_b200 import api
+    api._i8_torch()
+    from hearth_b200 import _pycall
     got = []
     vp, sz, i, fl = C.c_void_p, C.c_size_t, C.c_int, C.c_float
     kinds = [(vp, vp, sz, sz, vp), (vp, vp, vp, sz, vp, fl, sz, vp, sz, vp), (vp, vp, vp, sz, sz, vp), (vp, vp, sz, sz, vp), (vp, vp, sz, vp, sz, i, vp)]
     keep = [C.CFUNCTYPE(i, *k)(lambda *a: got.append(a) or len(got)) for k in kinds]
-    _pycall.bind(torch.float32, lambda device: 0x77 + device, *(C.cast(f, vp).value for f in keep))
+    _pycall.bind(*(C.cast(f, vp).value for f in keep))
     yield _pycall, got, torch
     api._F32 = None
     api._i8_torch()
     del keep
 
 
+class _Stream:
+    cuda_stream = 0x77
+
+
 def test_compiled_calls_pass_what_they_are_given(pycall):
     call, got, torch = pycall
-    f = torch.float32
-    x = _Tensor(f, (4, 96), (100, 1))
-    y = _Tensor(f, (5, 128), (100, 1), address=0x2000)
-    w = _Tensor(f, (96,), (1,), address=0x3000)
-    assert call.quantize(0x10, 0, 96, x, 4, None) == 1 and got[-1] == (0x10, 0x1000, 100, 4, 0x77)
-    assert call.dequantize(0x10, 0, 96, _Tensor(f, (1, 96), (1, 1)), 1, None) == 2 and got[-1] == (0x10, 0x1000, 96, 1, 0x77)
-    assert call.silu_mul(0x10, 0, 96, x, y, 4, None) == 3 and got[-1] == (0x10, 0x1000, 0x2000, 100, 4, 0x77)
-    assert call.add_rms_norm(0x10, 0, 96, x, y, w, 0.5, 4, None, None) == 4 and got[-1] == (0x10, 0x1000, 0x2000, 100, 0x3000, 0.5, 4, None, 0, 0x77)
-    assert call.add_rms_norm(0x10, 0, 96, x, None, w, 0.5, 4, y, None) == 5 and got[-1] == (0x10, 0x1000, None, 100, 0x3000, 0.5, 4, 0x2000, 100, 0x77)
-
-    class Stream:
-        cuda_stream = 0x99
-
-    assert call.matmul(0x20, 0x10, 1, 96, 4, _Tensor(f, (4, 96), (96, 1), device=1), True, Stream()) == 6
-    assert got[-1] == (0x20, 0x10, 4, 0x1000, 96, 1, 0x99)
+    st = _Stream()
+    x, y = torch.zeros(4, 100)[:, :96], torch.zeros(5, 128)[:, :100]
+    y100 = torch.zeros(500)[:500].view(5, 100)
+    w, one = torch.zeros(96), torch.zeros(1, 96)
+    X, Y, W = x.data_ptr(), y100.data_ptr(), w.data_ptr()
+    assert call.quantize(0x10, -1, 96, x, 4, st) == 1 and got[-1] == (0x10, X, 100, 4, 0x77)
+    assert call.dequantize(0x10, -1, 96, one.as_strided((1, 96), (1, 1)), 1, st) == 2 and got[-1] == (0x10, one.data_ptr(), 96, 1, 0x77)
+    assert call.silu_mul(0x10, -1, 96, x, y100, 4, st) == 3 and got[-1] == (0x10, X, Y, 100, 4, 0x77)
+    assert call.add_rms_norm(0x10, -1, 96, x, y100, w, 0.5, 4, None, st) == 4 and got[-1] == (0x10, X, Y, 100, W, 0.5, 4, None, 0, 0x77)
+    assert call.add_rms_norm(0x10, -1, 96, x, None, w, 0.5, 4, y, st) == 5 and got[-1] == (0x10, X, None, 100, W, 0.5, 4, y.data_ptr(), 128, 0x77)
+    assert call.matmul(0x20, 0x10, -1, 96, 4, x, True, st) == 6 and got[-1] == (0x20, 0x10, 4, X, 100, 1, 0x77)
+    empty = torch.zeros(0, 96)
+    assert call.quantize(0x10, -1, 96, empty, 0, st) == 7 and got[-1][2:4] == (96, 0)
 
 
 def test_compiled_calls_leave_everything_else_to_the_checks_in_python(pycall):
     call, got, torch = pycall
-    f = torch.float32
-    x, w = _Tensor(f, (4, 96), (96, 1)), _Tensor(f, (96,), (1,))
-    other = [None, 3, _Tensor(torch.float16, (4, 96), (96, 1)), _Tensor(f, (4, 96), (96, 1), device=1), _Tensor(f, (4, 96), (96, 1), device=-1),
-             _Tensor(f, (3, 96), (96, 1)), _Tensor(f, (4, 95), (96, 1)), _Tensor(f, (4, 96), (1, 4)), _Tensor(f, (96,), (1,)), _Tensor(f, (1, 4, 96), (384, 96, 1))]
+    st = _Stream()
+    x, w = torch.zeros(4, 96), torch.zeros(96)
+    other = [None, 3, x.half(), x.numpy(), torch.zeros(3, 96), torch.zeros(4, 95), torch.zeros(96, 4).t(), torch.zeros(96), torch.zeros(1, 4, 96), x.to_sparse(),
+             torch.zeros(4, 96, device="meta")]
     for t in other:
-        assert call.quantize(0x10, 0, 96, t, 4, None) is None
-        assert call.dequantize(0x10, 0, 96, t, 4, None) is None
-        assert call.silu_mul(0x10, 0, 96, t, x, 4, None) is None and call.silu_mul(0x10, 0, 96, x, t, 4, None) is None
-        assert call.add_rms_norm(0x10, 0, 96, t, None, w, 0.5, 4, None, None) is None
-        assert call.matmul(0x20, 0x10, 0, 96, 4, t, False, None) is None
+        assert call.quantize(0x10, -1, 96, t, 4, st) is None
+        assert call.dequantize(0x10, -1, 96, t, 4, st) is None
+        assert call.silu_mul(0x10, -1, 96, t, x, 4, st) is None and call.silu_mul(0x10, -1, 96, x, t, 4, st) is None
+        assert call.add_rms_norm(0x10, -1, 96, t, None, w, 0.5, 4, None, st) is None
+        assert call.matmul(0x20, 0x10, -1, 96, 4, t, False, st) is None
         if t is not None:
-            assert call.add_rms_norm(0x10, 0, 96, x, t, w, 0.5, 4, None, None) is None
-            assert call.add_rms_norm(0x10, 0, 96, x, None, w, 0.5, 4, t, None) is None
-    wide = _Tensor(f, (4, 96), (97, 1))
-    assert call.silu_mul(0x10, 0, 96, x, wide, 4, None) is None and call.add_rms_norm(0x10, 0, 96, x, wide, w, 0.5, 4, None, None) is None
-    assert call.add_rms_norm(0x10, 0, 96, x, None, x, 0.5, 4, None, None) is None and call.add_rms_norm(0x10, 0, 96, x, None, w, 1, 4, None, None) is None
-    assert call.quantize(0x10, 0, 96, x, -1, None) is None and call.quantize(0x10, 0, 96, x, 4, "stream") is None and call.quantize(0x10, 0, 96, x) is None
+            assert call.add_rms_norm(0x10, -1, 96, x, t, w, 0.5, 4, None, st) is None
+            assert call.add_rms_norm(0x10, -1, 96, x, None, w, 0.5, 4, t, st) is None
+    wide = torch.zeros(4, 97)
+    assert call.silu_mul(0x10, -1, 96, x, wide, 4, st) is None and call.add_rms_norm(0x10, -1, 96, x, wide, w, 0.5, 4, None, st) is None
+    assert call.add_rms_norm(0x10, -1, 96, x, None, x, 0.5, 4, None, st) is None and call.add_rms_norm(0x10, -1, 96, x, None, w, 1, 4, None, st) is None
+    assert call.quantize(0x10, 0, 96, x, 4, st) is None  # a CPU tensor where the handle lives on a GPU
+    assert call.quantize(0x10, -1, 96, x, -1, st) is None and call.quantize(0x10, -1, 96, x, 4, "stream") is None and call.quantize(0x10, -1, 96, x) is None
+    assert call.quantize(0x10, -1, 96, x, 4, None) is None
     assert not got
     with pytest.raises(TypeError):
-        call.bind(f, None, 0, 0, 0, 0, 0)
+        call.bind(0, 0, 0, 0, 0)
