@@ -15,9 +15,10 @@
 //
 // HBM-bound: 4 B (quantize, + 4 silu_mul, + 8 add_rms_norm) read or written per element and 1 B written.  One CTA per
 // row (a cluster of eight for a few long rows) keeps the row in registers between the reduction and the rounding, up to
-// 32 values a thread; many rows of more than 32768 columns are read twice.  Measured: quantize of 4096 x 4096 14.1 us
-// (5.9 TB/s), add_rms_norm 35 us (6.2 TB/s), silu_mul 30 us (5.0 TB/s: exp and the division take as long as the reads),
-// one row of 4096 columns 1.5 / 2.4 / 1.9 us behind its predecessor in a graph.
+// 32 values a thread; many rows of more than 32768 columns are read twice.  Measured: quantize of 4096 x 4096 13.7 us
+// (6.1 TB/s), add_rms_norm 36 us (6.1 TB/s), silu_mul 26 us (5.8 TB/s), of 512 x 17408 19.5 us (4.1 TB/s: two rows are all
+// that fit an SM's registers, and they load and compute in step), one row of 4096 columns 1.5 / 2.3 / 1.9 us behind its
+// predecessor in a graph.
 //
 // Reference counterparts with a scale per 32 columns: ops::rms_norm_q8 and ops::silu_mul_q8
 // (hearth-llm/src/ops.rs:273-306, :442-504), quantize_q8_0 (hearth-quant/src/q8_0.rs:20-51).
@@ -47,6 +48,7 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return __byte_perm(lo, hi, 0x5410);
 }
 
+// Columns c .. c + 3 of a row; zero past column n.
 template <bool VEC>
 __device__ __forceinline__ float4 read4(const float* row, int c, int n) {
     if (VEC) return c < n ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -57,10 +59,18 @@ __device__ __forceinline__ float4 read4(const float* row, int c, int n) {
     v.w = c + 3 < n ? row[c + 3] : 0.f;
     return v;
 }
-template <bool VEC>
+// STREAM: the lines are the first to leave L2 (see i8_stream_bytes).
+template <bool VEC, bool STREAM>
+__device__ __forceinline__ float4 read4(const float* row, int c, int n) {
+    if (VEC && STREAM) return c < n ? __ldcs(reinterpret_cast<const float4*>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return read4<VEC>(row, c, n);
+}
+template <bool VEC, bool STREAM>
 __device__ __forceinline__ void write4(float* row, int c, int n, float4 v) {
     if (VEC) {
-        if (c < n) *reinterpret_cast<float4*>(row + c) = v;
+        if (c >= n) return;
+        if (STREAM) __stcs(reinterpret_cast<float4*>(row + c), v);
+        else *reinterpret_cast<float4*>(row + c) = v;
         return;
     }
     if (c < n) row[c] = v.x;
@@ -81,15 +91,15 @@ __device__ __forceinline__ float4 mul4(float4 a, float4 b) {
 // The values v of N float4s of a row, `step` columns apart from column c (zero past the row's end or `limit`); the norm adds h * h to `sq`
 // and writes h.  All reads of the inputs come before the first write: the compiler may not move a read over a write
 // that could be to the same memory (the sum may overwrite an input), and reads one behind the other would leave HBM idle.
-template <int OP, bool VEC, int N>
+template <int OP, bool VEC, bool STREAM, int N>
 __device__ __forceinline__ void values(const I8Rows& p, size_t row, int c, int step, int limit, float4 (&v)[N], float& sq) {
     const int n = min(p.n_cols, limit);
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = read4<VEC>(p.x + row * p.ld, c + i * step, n);
+    for (int i = 0; i < N; i++) v[i] = read4<VEC, STREAM>(p.x + row * p.ld, c + i * step, n);
     if constexpr (OP != I8_QUANTIZE) if (OP == I8_SILU_MUL || p.y) {
         float4 y[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) y[i] = read4<VEC>(p.y + row * p.ld, c + i * step, n);
+        for (int i = 0; i < N; i++) y[i] = read4<VEC, STREAM>(p.y + row * p.ld, c + i * step, n);
 #pragma unroll
         for (int i = 0; i < N; i++) {
             if constexpr (OP == I8_SILU_MUL)
@@ -101,7 +111,7 @@ __device__ __forceinline__ void values(const I8Rows& p, size_t row, int c, int s
     if constexpr (OP == I8_ADD_RMS_NORM) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (p.sum) write4<VEC>(p.sum + row * p.ld_sum, c + i * step, n, v[i]);
+            if (p.sum) write4<VEC, false>(p.sum + row * p.ld_sum, c + i * step, n, v[i]);
             sq = fmaf(v[i].x, v[i].x, sq);
             sq = fmaf(v[i].y, v[i].y, sq);
             sq = fmaf(v[i].z, v[i].z, sq);
@@ -120,7 +130,7 @@ __device__ __forceinline__ float4 value_again(const I8Rows& p, size_t row, int c
         return mul4(read4<VEC>(p.weight, c, p.n_cols), read4<VEC>(p.sum + row * p.ld_sum, c, p.n_cols));
     float unused = 0.f;
     float4 v[1];
-    values<OP, VEC, 1>(p, row, c, 0, limit, v, unused);
+    values<OP, VEC, false, 1>(p, row, c, 0, limit, v, unused);
     return v[0];
 }
 
@@ -145,7 +155,7 @@ __device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
 
 // One CTA per row, or (CLUSTER) the CTAs of a cluster, each with a run of `quads` float4s of it.  NV = float4s of the row a
 // thread keeps (0: the row is read twice).
-template <int OP, int NV, bool VEC, bool CLUSTER, int MAX_THREADS, int MIN_CTAS>
+template <int OP, int NV, bool VEC, bool STREAM, bool CLUSTER, int MAX_THREADS, int MIN_CTAS>
 __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8Rows p, int quads) {
     __shared__ uint32_t s_max[32];
     __shared__ float s_sq[32];
@@ -158,18 +168,18 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS) i8_rows_kernel(const I8
     pdl_trigger();
     if (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's memory is there
     pdl_wait();
-    constexpr int BATCH = NV >= 4 ? 4 : (NV > 0 ? NV : 1), BATCHES = NV > 0 ? NV / BATCH : 1;
+    constexpr int BATCH = NV == 8 && OP == I8_ADD_RMS_NORM ? 2 : NV >= 4 ? 4 : (NV > 0 ? NV : 1), BATCHES = NV > 0 ? NV / BATCH : 1;
     float4 v[BATCHES][BATCH];
     uint32_t m = 0;
     float sq = 0.f;
     if (NV > 0) {
 #pragma unroll
-        for (int b = 0; b < BATCHES; b++) values<OP, VEC, BATCH>(p, row, c0 + b * BATCH * step, step, padded, v[b], sq);
+        for (int b = 0; b < BATCHES; b++) values<OP, VEC, STREAM, BATCH>(p, row, c0 + b * BATCH * step, step, padded, v[b], sq);
 #pragma unroll
         for (int i = 0; i < NV; i++) m = absmax4(m, v[i / BATCH][i % BATCH]);
     } else {
         for (int c = c0; c < padded; c += step) {
-            values<OP, VEC, BATCH>(p, row, c, 0, padded, v[0], sq);
+            values<OP, VEC, STREAM, BATCH>(p, row, c, 0, padded, v[0], sq);
             m = absmax4(m, v[0][0]);
         }
     }
@@ -296,7 +306,7 @@ __global__ void __launch_bounds__(128) i8_store_kernel(I8Plane plane, const floa
 
 // Plane -> the f32 values it stands for, q * scale.  A thread takes four columns of a group of eight rows: its eight loads
 // are in flight together (one row a thread ran at 2.4 TB/s).
-template <bool VEC>
+template <bool VEC, bool STREAM>
 __global__ void __launch_bounds__(128) i8_dequantize_kernel(I8Plane plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld) {
     pdl_trigger();
     pdl_wait();
@@ -316,9 +326,16 @@ __global__ void __launch_bounds__(128) i8_dequantize_kernel(I8Plane plane, const
         if (i >= rows) break;
         const float4 f = make_float4(__fmul_rn((float)(int8_t)(v[i]), s[i]), __fmul_rn((float)(int8_t)(v[i] >> 8), s[i]),
                                      __fmul_rn((float)(int8_t)(v[i] >> 16), s[i]), __fmul_rn((float)(int8_t)(v[i] >> 24), s[i]));
-        write4<VEC>(out + (size_t)(row0 + i) * ld, c, n_cols, f);
+        write4<VEC, STREAM>(out + (size_t)(row0 + i) * ld, c, n_cols, f);
     }
 }
+
+// From this many bytes of row-major input (or output) on, the lines a call touches are marked as the first to leave L2: they
+// would push out the 8-bit rows that the next kernel reads, and each other before anybody reads them again.  Measured with
+// the values read back behind it, us without and with: silu_mul of 4096 x 4096 40.1 / 37.6, of 512 x 17408 28.9 / 27.6, of 2048 x
+// 2048 14.4 / 13.9, norm of 4096 x 4096 48.3 / 47.2 (the norm alone 35.1 / 36.0).  Below, a set that stays in L2 between calls
+// would lose by it: silu_mul of 512 x 4096 9.4 / 10.8.
+constexpr size_t i8_stream_bytes = 32u << 20;
 
 bool vec_rows(const void* p, size_t ld) { return ((reinterpret_cast<uintptr_t>(p) & 15) == 0) && (ld % 4 == 0); }
 
@@ -343,19 +360,22 @@ int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, in
 }
 
 template <int OP, int NV, int MAX_THREADS, int MIN_CTAS>
-int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, cudaStream_t st) {
-    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, false, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, false, MAX_THREADS, MIN_CTAS>,
+int launch_rows_nv(const I8Rows& p, int n_rows, int threads, bool vec, bool stream, cudaStream_t st) {
+    constexpr bool CAN = NV >= 4;  // so many bytes come with at least four float4s a thread, or with rows that are read twice
+    return launch_pdl(!vec     ? i8_rows_kernel<OP, NV, false, false, false, MAX_THREADS, MIN_CTAS>
+                      : stream ? i8_rows_kernel<OP, NV, true, CAN, false, MAX_THREADS, MIN_CTAS>
+                               : i8_rows_kernel<OP, NV, true, false, false, MAX_THREADS, MIN_CTAS>,
                       dim3(n_rows), threads, st, 1, p, I8_MAX_COLS / 4);
 }
 template <int OP, int NV, int MAX_THREADS, int MIN_CTAS>
 int launch_rows_cluster(const I8Rows& p, int n_rows, int ctas, int quads, bool vec, cudaStream_t st) {
     const int threads = ((quads + NV - 1) / NV + 31) / 32 * 32;
-    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, true, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, true, MAX_THREADS, MIN_CTAS>,
+    return launch_pdl(vec ? i8_rows_kernel<OP, NV, true, false, true, MAX_THREADS, MIN_CTAS> : i8_rows_kernel<OP, NV, false, false, true, MAX_THREADS, MIN_CTAS>,
                       dim3(ctas, n_rows), threads, st, ctas, p, quads);
 }
 
 template <int OP>
-int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
+int launch_rows_op(const I8Rows& p, int n_rows, bool vec, bool stream, cudaStream_t st) {
     const int quads = ((p.n_cols + 127) & ~127) / 4;  // float4s of a padded row
     const auto threads = [&](int nv) { return ((quads + nv - 1) / nv + 31) / 32 * 32; };
     // Few rows: as few float4s a thread as still leave all rows resident at once (latency).  Many rows: four or eight, so
@@ -370,13 +390,16 @@ int launch_rows_op(const I8Rows& p, int n_rows, bool vec, cudaStream_t st) {
         if (part <= 1024) return launch_rows_cluster<OP, 1, 1024, 1>(p, n_rows, 8, part, vec, st);
         return launch_rows_cluster<OP, 2, 1024, 1>(p, n_rows, 8, part, vec, st);
     }
-    if (resident(1)) return launch_rows_nv<OP, 1, 1024, 1>(p, n_rows, threads(1), vec, st);
-    if (resident(2)) return launch_rows_nv<OP, 2, 1024, 1>(p, n_rows, threads(2), vec, st);
-    if (threads(4) <= 512) return launch_rows_nv<OP, 4, 512, 2>(p, n_rows, threads(4), vec, st);
-    if (threads(4) <= 1024 && resident(4)) return launch_rows_nv<OP, 4, 1024, 1>(p, n_rows, threads(4), vec, st);
-    if (threads(8) <= 576) return launch_rows_nv<OP, 8, 576, 2>(p, n_rows, threads(8), vec, st);
-    if (threads(8) <= 1024) return launch_rows_nv<OP, 8, 1024, 1>(p, n_rows, threads(8), vec, st);
-    return launch_rows_nv<OP, 0, 1024, 1>(p, n_rows, 1024, vec, st);
+    if (resident(1)) return launch_rows_nv<OP, 1, 1024, 1>(p, n_rows, threads(1), vec, stream, st);
+    if (resident(2)) return launch_rows_nv<OP, 2, 1024, 1>(p, n_rows, threads(2), vec, stream, st);
+    // (48 registers: five CTAs of 256 threads or four of 320 per SM; silu_mul of 4096 x 4096 26.2 us, with 56 and four 30.9)
+    if (threads(4) <= 256) return launch_rows_nv<OP, 4, 256, 5>(p, n_rows, threads(4), vec, stream, st);
+    if (threads(4) <= 320) return launch_rows_nv<OP, 4, 320, 4>(p, n_rows, threads(4), vec, stream, st);
+    if (threads(4) <= 512) return launch_rows_nv<OP, 4, 512, 2>(p, n_rows, threads(4), vec, stream, st);
+    if (threads(4) <= 1024 && resident(4)) return launch_rows_nv<OP, 4, 1024, 1>(p, n_rows, threads(4), vec, stream, st);
+    if (threads(8) <= 576) return launch_rows_nv<OP, 8, 576, 2>(p, n_rows, threads(8), vec, stream, st);
+    if (threads(8) <= 1024) return launch_rows_nv<OP, 8, 1024, 1>(p, n_rows, threads(8), vec, stream, st);
+    return launch_rows_nv<OP, 0, 1024, 1>(p, n_rows, 1024, vec, stream, st);
 }
 
 dim3 move_grid(int n_rows, int n_cols) {
@@ -388,14 +411,15 @@ dim3 move_grid(int n_rows, int n_cols) {
 
 int launch_i8_rows(int op, const I8Rows& p, int n_rows, cudaStream_t st) {
     if (n_rows <= 0) return 0;
+    const bool stream = (size_t)n_rows * p.n_cols * sizeof(float) * (p.y ? 2 : 1) >= i8_stream_bytes;
     bool vec = (p.n_cols % 4 == 0) && vec_rows(p.x, p.ld);
     if (p.y) vec = vec && vec_rows(p.y, p.ld);
     if (p.weight) vec = vec && vec_rows(p.weight, 0);
     if (p.sum) vec = vec && vec_rows(p.sum, p.ld_sum);
     switch (op) {
-        case I8_QUANTIZE: return launch_rows_op<I8_QUANTIZE>(p, n_rows, vec, st);
-        case I8_SILU_MUL: return launch_rows_op<I8_SILU_MUL>(p, n_rows, vec, st);
-        default: return launch_rows_op<I8_ADD_RMS_NORM>(p, n_rows, vec, st);
+        case I8_QUANTIZE: return launch_rows_op<I8_QUANTIZE>(p, n_rows, vec, stream, st);
+        case I8_SILU_MUL: return launch_rows_op<I8_SILU_MUL>(p, n_rows, vec, stream, st);
+        default: return launch_rows_op<I8_ADD_RMS_NORM>(p, n_rows, vec, stream, st);
     }
 }
 
@@ -412,8 +436,9 @@ int launch_i8_store(const I8Plane& plane, const float* scales, int n_rows, int n
 int launch_i8_dequantize(const I8Plane& plane, const float* scales, int n_rows, int n_cols, float* out, size_t ld, cudaStream_t st) {
     if (n_rows <= 0) return 0;
     const dim3 grid((n_cols + 511) / 512, (n_rows + 7) / 8);
-    const bool vec = (n_cols % 4 == 0) && vec_rows(out, ld);
-    return launch_pdl(vec ? i8_dequantize_kernel<true> : i8_dequantize_kernel<false>, grid, 128, st, 1, plane, scales, n_rows, n_cols, out, ld);
+    const bool vec = (n_cols % 4 == 0) && vec_rows(out, ld), stream = (size_t)n_rows * n_cols * sizeof(float) >= i8_stream_bytes;
+    return launch_pdl(!vec ? i8_dequantize_kernel<false, false> : stream ? i8_dequantize_kernel<true, true> : i8_dequantize_kernel<true, false>, grid, 128, st,
+                      1, plane, scales, n_rows, n_cols, out, ld);
 }
 
 }  // namespace hb200
