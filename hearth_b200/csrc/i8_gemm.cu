@@ -38,6 +38,8 @@ namespace {
 constexpr int W_TILE = 16384;  // 128 rows x 128 bytes
 constexpr int MAX_SPLIT = 8;   // portable cluster size
 
+// Only once this CTA has its TMEM: a dependent kernel's CTA that came first to the SM's columns would wait for this grid's end, and
+// this one for the columns.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -160,7 +162,6 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     const int8_t* wp = p.w + ((size_t)row_tile * p.kb + k0) * W_TILE;
     const int8_t* xp = p.a + (size_t)k0 * p.a_kb_stride + (size_t)tok0 * 128;
 
-    pdl_trigger();
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full[s]), 1);
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(128) i8_split_kernel(const I8Product p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_trigger();
     pdl_wait();
 
     if (warp == 0) {
@@ -423,7 +425,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     const auto w_src = [&](const PairTile& t) { return p.w + (size_t)min(t.row_tile, last_row_tile) * p.kb * W_TILE; };
     const auto x_src = [&](const PairTile& t) { return p.a + (size_t)(t.tok0 + (int)rank * (NT / 2)) * 128; };
 
-    pdl_trigger();
     const PairTile t0 = pair_tile<NT>(pair, row_pairs, tok_tiles, rank);
     const int steps = (p.kb + 1) / 2;     // stages of a tile
     const int ahead = min(steps, STAGES);  // stages whose weights are fetched before the wait on the previous kernel
@@ -455,6 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     cluster_sync();  // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_trigger();
     pdl_wait();
 
     if (warp == 0) {
