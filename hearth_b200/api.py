@@ -466,7 +466,10 @@ def _i8_torch() -> None:
     if _F32 is not None:
         return
     import torch
-    from . import _pycall
+    try:
+        from . import _pycall
+    except ImportError as e:
+        raise ImportError("hearth_b200/_pycall.so is missing or was built for another torch: build it with `python -m hearth_b200.build`") from e
     L = _l.load()
     raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
     hot = ("hb200_act_i8_quantize_dev", "hb200_act_i8_add_rms_norm_dev", "hb200_act_i8_silu_mul_dev", "hb200_act_i8_dequantize_dev",

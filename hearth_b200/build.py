@@ -44,11 +44,17 @@ def _headers() -> list[str]:
 PYCALL = os.path.join(HERE, "_pycall.so")
 
 
-def build_pycall(force: bool = False) -> str:
+def build_pycall(force: bool = False) -> str | None:
+    """None where there is no torch with CUDA: the calls it serves take CUDA tensors."""
     src = os.path.join(CSRC, "pycall.cpp")
     if force or _stale(PYCALL, [src]):
-        import torch
+        try:
+            import torch
+        except ImportError:
+            return None
         root = os.path.dirname(torch.__file__)
+        if not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
+            return None
         cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
         include = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                    os.path.join(cuda, "include")]

@@ -418,7 +418,8 @@ HB200_API int hb200_act_i8_quantize_dev(hb200_act_i8_t a, const float *x_dev, si
 /* The residual's addition and the norm in front of a projection: h = x + residual (residual_dev may be null: h = x; its
  * rows are ld_x apart, too), written to sum_dev unless that is null (sum_dev may be x_dev or residual_dev, then with
  * ld_sum = ld_x); then v = weight * h is rounded to 8 bits and its scale multiplied by 1 / sqrt(mean(h^2) + eps).
- * The integers therefore do not depend on how the mean is summed.  eps > 0.  h^2 has to stay in the range of f32. */
+ * The integers therefore do not depend on how the mean is summed.  eps > 0.  The sum of h^2 has to stay in the range of f32
+ * (a row where it does not gets scale NaN). */
 HB200_API int hb200_act_i8_add_rms_norm_dev(hb200_act_i8_t a, const float *x_dev, const float *residual_dev, size_t ld_x,
                                             const float *weight_dev, float eps, size_t seq_len, float *sum_dev,
                                             size_t ld_sum, void *stream);
