@@ -196,6 +196,23 @@ int encode_qmap(hb200_act* a) {
     return 0;
 }
 
+}  // namespace
+namespace hb200 {
+int encode_i8_plane(void* map, const int8_t* q, size_t rows, size_t blocks, size_t block_stride, int box_rows) {
+    const cuuint64_t dims[3] = {128, (cuuint64_t)rows, (cuuint64_t)blocks};
+    const cuuint64_t strides[2] = {128, (cuuint64_t)block_stride};
+    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    // no swizzle: the plane is stored swizzled
+    const CUresult r = g_encode_tiled(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(q), dims, strides, box, estr,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with code %d", (int)r); return HB200_ERR_CUDA; }
+    return 0;
+}
+}  // namespace hb200
+namespace {
+
 int kind_of(int dtype) {
     switch (dtype) {
         case HB200_Q1_0: case HB200_Q1_0_G128: case HB200_Q1_0_G128_LEGACY: return KIND_Q1;

@@ -373,10 +373,14 @@ struct I8Product {
     int n_rows, n_tok, kb;
     int accumulate;       // out += result
     int* status;          // device word for an expired wait
+    const void *w_map, *x_map_n128, *x_map_n256;  // host: tensor maps of the planes (encode_i8_plane); boxes of 128 rows, of 64 and of 128 tokens
 };
 int i8_gemm_prepare(int sm_count);  // per device: kernel attributes, clusters that fit at once
 int launch_i8_gemm(const I8Product& p, cudaStream_t st);
 const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok);
+// abi.cu: the tensor map (a CUtensorMap) of `blocks` 128-column blocks of `rows` rows, block_stride bytes apart, boxes of one block and
+// box_rows rows; the rows behind a block's last one read as zeros.
+int encode_i8_plane(void* map, const int8_t* q, size_t rows, size_t blocks, size_t block_stride, int box_rows);
 // i8_abi.cu: frees what the host-buffer product keeps for a slot.
 void i8_release_slot(int slot);
 

@@ -18,6 +18,7 @@ struct hb200_weight_i8 {
     I8Plane plane = {};
     float* scales = nullptr;
     size_t resident_bytes = 0;
+    CUtensorMap map;  // one 128-row tile of one block
 };
 struct hb200_act_i8 {
     int slot = 0, device = 0;
@@ -25,6 +26,7 @@ struct hb200_act_i8 {
     int kb = 0;
     I8Plane plane = {};
     float* scales = nullptr;
+    CUtensorMap map64, map128;  // 64 and 128 tokens of one block
 };
 
 namespace {
@@ -137,6 +139,12 @@ int weight_new(size_t n_rows, size_t n_cols, hb200_weight_i8** out) {
             return HB200_ERR_CUDA;
         }
         w->scales = reinterpret_cast<float*>(w->plane.q + bytes);
+        const int rc = encode_i8_plane(&w->map, w->plane.q, 128, tiles * w->kb, 16384, 128);
+        if (rc) {
+            cudaFree(w->plane.q);
+            delete w;
+            return rc;
+        }
     }
     *out = w;
     return 0;
@@ -208,6 +216,9 @@ int product(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, float* out, s
     p.kb = w->kb;
     p.accumulate = accumulate != 0;
     p.status = slot_status();
+    p.w_map = &w->map;
+    p.x_map_n128 = &a->map64;
+    p.x_map_n256 = &a->map128;
     return launch_i8_gemm(p, st);
 }
 
@@ -343,6 +354,13 @@ extern "C" int hb200_act_i8_create(size_t max_seq_len, size_t n_cols, hb200_act_
         return HB200_ERR_CUDA;
     }
     a->scales = reinterpret_cast<float*>(a->plane.q + bytes);
+    rc = encode_i8_plane(&a->map64, a->plane.q, groups * 8, a->kb, a->plane.kb_stride, 64);
+    if (!rc) rc = encode_i8_plane(&a->map128, a->plane.q, groups * 8, a->kb, a->plane.kb_stride, 128);
+    if (rc) {
+        cudaFree(a->plane.q);
+        delete a;
+        return rc;
+    }
     *out = a;
     return HB200_OK;
     I8_END

@@ -4,7 +4,7 @@
 // The weight rows are the MMA's M (128 TMEM lanes), the tokens its N (TMEM columns): tcgen05.mma kind::i8, 128 x NTOK x 32.
 // With the channel on the lane a warp's store of one token is 128 contiguous bytes, and a short batch costs no more
 // than its own columns.  Both planes are stored as swizzled shared-memory tiles (common.cuh), so an operand is one
-// contiguous bulk copy: 16 KiB of weights and NTOK * 128 bytes of activations per 128-column block, no tensor map.
+// contiguous copy: 16 KiB of weights and NTOK * 128 bytes of activations per 128-column block.
 //
 // Few tokens: the time is the weights' way from HBM, and what counts is how many bytes are in flight on how many SMs.
 // A tile of 128 rows is cut along K over the CTAs of a cluster; integer partial sums meet through distributed shared
@@ -14,7 +14,8 @@
 //
 // Many tokens: bound by the tensor cores, so a pair of CTAs works on one tile of 256 rows x NT tokens (cta_group::2: each
 // SM holds half of either operand, which halves the shared-memory traffic per product), persistent over the tiles, two
-// accumulators in TMEM so that one tile is scaled and stored while the next is summed.
+// accumulators in TMEM so that one tile is scaled and stored while the next is summed.  Its copies go through tensor maps (made
+// with the handles): of a copy's forms only that one may count its bytes at a barrier of the other CTA of the pair.
 //
 // Measured (back to back in a graph, us; weight bytes per second or operations per second):
 //   1 x 2048 x 151669   47.0 (6.6 TB/s, the copy bandwidth)      4 x 5120 x 34816    27.5 (6.5 TB/s)
@@ -96,6 +97,28 @@ __device__ __forceinline__ void peer_st4(uint32_t addr, uint32_t a, uint32_t b, 
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
         if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if ((i & 7) == 7 && __any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    *abort_flag = 1;
+    atomicCAS(status, 0, code);
+    return false;
+}
+
+// The same with acquire at cluster scope, for barriers that the other CTA of a pair (or its copies) arrives at.
+__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
+        if (__all_sync(0xffffffffu, mbar_try_cluster(bar, parity))) return true;
         if ((i & 7) == 7 && __any_sync(0xffffffffu, *abort_flag)) return false;
     }
     *abort_flag = 1;
@@ -317,8 +340,8 @@ template <int NT>
 struct PairCfg {
     static constexpr int X_TILE = NT / 2 * 128;  // this CTA's half of the tokens
     // Two 128-column blocks a stage (the last stage of a tile may hold one): a barrier test costs the issuing warp some
-    // 160 cycles even when it succeeds, and a stage has two of them; with one block a stage (256 cycles of MMAs at 128
-    // tokens) the tensor pipe waited for the issue.
+    // 160 cycles even when it succeeds; with one block a stage (256 cycles of MMAs at 128 tokens) the tensor pipe waited
+    // for the issue.
     static constexpr int STAGE = 2 * (W_TILE + X_TILE);
     static constexpr int STAGES = NT == 256 ? 3 : 4;
     static constexpr int SMEM = STAGES * STAGE + 1024;
@@ -330,11 +353,18 @@ constexpr int PAIR_THREADS = 32 * (2 + PAIR_EPI_WARPS);  // producer, MMA issue 
 // 17408 columns are 71 MB), and the weights are read once per group.
 constexpr int TOK_GROUP = 16;
 
-// Arrival at a barrier of the other CTA.  Neither side needs a fence for plain memory (with .release / .acquire.cluster on
-// this pair a stage took a microsecond): what the barrier orders are bulk copies and tensor-core reads of shared
-// memory, and TMEM reads, which tcgen05.fence covers.
+// A block of 128 columns of a plane, rows `row` .. of the map's box, into this CTA's memory; its bytes count at `bar`, a barrier of
+// either CTA of the pair.  What a copy wrote is visible to whoever acquires the completed phase at cluster scope, so the
+// leader's one barrier per stage covers both CTAs' halves of it.
+__device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap* map, int row, int block, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(row), "r"(block), "r"(bar)
+        : "memory");
+}
+// Arrival at a barrier of the other CTA, released at cluster scope.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -398,14 +428,14 @@ __device__ __forceinline__ PairTile pair_tile(int t, int row_pairs, int tok_tile
 }
 
 template <int NT, bool ACC>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_pair_kernel(const I8Product p, int row_pairs, int tok_tiles) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    i8_pair_kernel(const I8Product p, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, int row_pairs, int tok_tiles) {
     using C = PairCfg<NT>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ unsigned char dyn[];
-    // full: this CTA's copies of a stage; peer_full (leader): the other CTA's; empty: the stage may be refilled;
-    // acc_full / acc_empty: an accumulator is complete / has been read (leader: by both CTAs' epilogue warps); drained: no
-    // MMA is under way any more
-    __shared__ uint64_t full[STAGES], peer_full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
+    // full (leader): both CTAs' copies of a stage; empty: the stage may be refilled; acc_full / acc_empty: an accumulator is
+    // complete / has been read (leader: by both CTAs' epilogue warps); drained: no MMA is under way any more
+    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -414,16 +444,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, n_tiles = row_pairs * tok_tiles;
     const int last_row_tile = (p.n_rows + 127) / 128 - 1;
     const uint32_t ring = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t full0 = smem_u32(&full[0]), empty0 = smem_u32(&empty[0]);
 
-    const uint32_t full0 = smem_u32(&full[0]), peer0 = smem_u32(&peer_full[0]), empty0 = smem_u32(&empty[0]);
-
-    // What stage `it` of this CTA holds: weights and tokens of block k of tile t, and their bytes.
-    const auto x_bytes = [&](int tok0) {
-        const int left = p.n_tok - (tok0 + (int)rank * (NT / 2));
-        return left <= 0 ? 0u : (uint32_t)((min(left, NT / 2) + 7) / 8) * 1024u;
+    // Rank r's half of a tile's tokens: none of them may be there, else a whole box is read (rows behind the plane's are zeros).
+    const auto half_live = [&](int tok0, int r) { return tok0 + r * (NT / 2) < p.n_tok; };
+    const auto stage_bytes = [&](int tok0, int blocks) {  // of both CTAs
+        return (uint32_t)blocks * (2 * W_TILE + (half_live(tok0, 1) ? 2 : 1) * C::X_TILE);
     };
-    const auto w_src = [&](const PairTile& t) { return p.w + (size_t)min(t.row_tile, last_row_tile) * p.kb * W_TILE; };
-    const auto x_src = [&](const PairTile& t) { return p.a + (size_t)(t.tok0 + (int)rank * (NT / 2)) * 128; };
+    const auto w_block = [&](const PairTile& t) { return min(t.row_tile, last_row_tile) * p.kb; };
 
     const PairTile t0 = pair_tile<NT>(pair, row_pairs, tok_tiles, rank);
     const int steps = (p.kb + 1) / 2;     // stages of a tile
@@ -431,7 +459,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&peer_full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
         for (int a = 0; a < 2; a++) {
@@ -441,11 +468,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         mbar_init(smem_u32(&drained), 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int k = 0; k < ahead; k++) {
-            const uint32_t blocks = min(2, p.kb - 2 * k);
-            mbar_expect_tx(full0 + k * 8, blocks * (W_TILE + x_bytes(t0.tok0)));
-            bulk_load(ring + k * C::STAGE, w_src(t0) + (size_t)k * 2 * W_TILE, blocks * W_TILE, full0 + k * 8);
-        }
     }
     __syncwarp();
     if (warp == 1) {
@@ -456,6 +478,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
     cluster_sync();  // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    const uint32_t leader_full0 = peer_smem(full0, 0);
+    if (warp == 0 && elect_one()) {
+        for (int k = 0; k < ahead; k++) {
+            const int blocks = min(2, p.kb - 2 * k);
+            if (rank == 0) mbar_expect_tx(full0 + k * 8, stage_bytes(t0.tok0, blocks));
+            for (int b = 0; b < blocks; b++)
+                pair_load(ring + k * C::STAGE + b * W_TILE, &w_map, 0, w_block(t0) + 2 * k + b, leader_full0 + k * 8);
+        }
+    }
+    __syncwarp();
     pdl_trigger();
     pdl_wait();
 
@@ -465,84 +497,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += pairs) {
             const PairTile tl = pair_tile<NT>(t, row_pairs, tok_tiles, rank);
-            const uint32_t xb = x_bytes(tl.tok0);
-            const int8_t *ws = w_src(tl), *xs = x_src(tl);
+            const bool live = half_live(tl.tok0, rank);
+            const int w0 = w_block(tl), x_row = tl.tok0 + (int)rank * (NT / 2);
             for (int k = 0; k < p.kb; k += 2, it++) {
-                if (it >= STAGES) ok = mbar_wait_warp(empty0 + s * 8, phase, &abort_flag, p.status, 63);
+                if (it >= STAGES) ok = mbar_wait_pair(empty0 + s * 8, phase, &abort_flag, p.status, 63);
                 if (!ok) break;
                 if (elect_one()) {
-                    const uint32_t dst = ring + s * C::STAGE, bar = full0 + s * 8;
-                    const uint32_t blocks = min(2, p.kb - k);
+                    const uint32_t dst = ring + s * C::STAGE, bar = leader_full0 + s * 8;
+                    const int blocks = min(2, p.kb - k);
                     if (it >= ahead) {
-                        mbar_expect_tx(bar, blocks * (W_TILE + xb));
-                        bulk_load(dst, ws, blocks * W_TILE, bar);
+                        if (rank == 0) mbar_expect_tx(full0 + s * 8, stage_bytes(tl.tok0, blocks));
+                        pair_load(dst, &w_map, 0, w0 + k, bar);
+                        if (blocks == 2) pair_load(dst + W_TILE, &w_map, 0, w0 + k + 1, bar);
                     }
-                    if (xb) {
-                        bulk_load(dst + 2 * W_TILE, xs, xb, bar);
-                        if (blocks == 2) bulk_load(dst + 2 * W_TILE + C::X_TILE, xs + p.a_kb_stride, xb, bar);
+                    if (live) {
+                        pair_load(dst + 2 * W_TILE, &x_map, x_row, k, bar);
+                        if (blocks == 2) pair_load(dst + 2 * W_TILE + C::X_TILE, &x_map, x_row, k + 1, bar);
                     }
                 }
                 __syncwarp();
-                ws += 2 * W_TILE;
-                xs += 2 * p.a_kb_stride;
                 if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
-        if (*(volatile int*)&abort_flag) {  // nothing may still be on its way into this CTA's memory when it ends
+        // Nothing may still be on its way into either CTA's memory when they end: both stay until the leader has seen the copies land
+        // (a stage that the other CTA never filled runs into the limit).
+        if (rank == 0 && *(volatile int*)&abort_flag) {
             for (int i = max(0, it - STAGES); i < it; i++)
-                for (uint32_t n = 0; n < SPIN_LIMIT && !mbar_try(full0 + i % STAGES * 8, (uint32_t)(i / STAGES) & 1u); n++) {}
+                for (uint32_t n = 0; n < SPIN_LIMIT && !mbar_try_cluster(full0 + i % STAGES * 8, (uint32_t)(i / STAGES) & 1u); n++) {}
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         // D = S32, A and B signed int8, both K-major, M = 256 over the pair, N = NT
         constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
         const uint64_t ad0 = make_desc(ring), bd0 = make_desc(ring + 2 * W_TILE);
-        const uint32_t leader_full0 = peer_smem(smem_u32(&peer_full[0]), 0);
         int n = 0, s = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += pairs, n++) {
             const int a = n & 1;
-            if (rank == 0 && n >= 2) {
-                ok = mbar_wait_warp(smem_u32(&acc_empty[a]), (uint32_t)(n / 2 - 1) & 1u, &abort_flag, p.status, 64);
+            if (n >= 2) {
+                ok = mbar_wait_pair(smem_u32(&acc_empty[a]), (uint32_t)(n / 2 - 1) & 1u, &abort_flag, p.status, 64);
                 if (!ok) break;
                 tc_fence_after();
             }
             for (int k = 0; k < p.kb; k += 2) {
-                ok = mbar_wait_warp(full0 + s * 8, phase, &abort_flag, p.status, 65);
+                ok = mbar_wait_pair(full0 + s * 8, phase, &abort_flag, p.status, 65);
                 if (!ok) break;
-                if (rank != 0) {  // tell the leader that this half of the stage has landed
-                    if (elect_one()) mbar_arrive_remote(leader_full0 + s * 8);
-                    __syncwarp();
-                } else {
-                    ok = mbar_wait_warp(peer0 + s * 8, phase, &abort_flag, p.status, 66);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t ad = ad0 + (uint32_t)(s * (C::STAGE >> 4)), bd = bd0 + (uint32_t)(s * (C::STAGE >> 4));
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t ad = ad0 + (uint32_t)(s * (C::STAGE >> 4)), bd = bd0 + (uint32_t)(s * (C::STAGE >> 4));
 #pragma unroll
-                        for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
-                        if (k + 1 < p.kb) {
+                    for (int j = 0; j < 4; j++) mma_i8_pair(tmem + a * NT, ad + 2 * j, bd + 2 * j, IDESC, (k | j) != 0);
+                    if (k + 1 < p.kb) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                mma_i8_pair(tmem + a * NT, ad + (W_TILE >> 4) + 2 * j, bd + (C::X_TILE >> 4) + 2 * j, IDESC, 1);
-                        }
-                        commit_pair(empty0 + s * 8);
-                        if (k + 2 >= p.kb) commit_pair(smem_u32(&acc_full[a]));
+                        for (int j = 0; j < 4; j++)
+                            mma_i8_pair(tmem + a * NT, ad + (W_TILE >> 4) + 2 * j, bd + (C::X_TILE >> 4) + 2 * j, IDESC, 1);
                     }
-                    __syncwarp();
+                    commit_pair(empty0 + s * 8);
+                    if (k + 2 >= p.kb) commit_pair(smem_u32(&acc_full[a]));
                 }
+                __syncwarp();
                 if (++s == STAGES) { s = 0; phase ^= 1; }
             }
         }
         // also after a wait that ran out: no MMA may still read either CTA's memory when they end
-        if (rank == 0 && elect_one()) commit_pair(smem_u32(&drained));
+        if (elect_one()) commit_pair(smem_u32(&drained));
         __syncwarp();
-        await_mmas(smem_u32(&drained));
-    } else {
+    } else if (warp >= 2) {
         const int q = warp & 3;                      // TMEM lane quarter of this warp
         const int half = (warp - 2) / 4 * (NT / 2);  // its first token of the tile
-        const uint32_t leader_empty[2] = {peer_smem(smem_u32(&acc_empty[0]), 0), peer_smem(smem_u32(&acc_empty[1]), 0)};
+        const uint32_t leader_empty0 = peer_smem(smem_u32(&acc_empty[0]), 0);
         int n = 0;
         for (int t = pair; t < n_tiles; t += pairs, n++) {
             const int a = n & 1;
@@ -550,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
             const int row = tl.row_tile * 128 + q * 32 + lane;
             const bool live = row < p.n_rows;
             const float sw = live ? p.sw[row] : 0.f;
-            if (!mbar_wait_warp(smem_u32(&acc_full[a]), (uint32_t)(n / 2) & 1u, &abort_flag, p.status, 67)) break;
+            if (!mbar_wait_pair(smem_u32(&acc_full[a]), (uint32_t)(n / 2) & 1u, &abort_flag, p.status, 67)) break;
             tc_fence_after();
             const uint32_t tm = tmem + a * NT + half + ((uint32_t)(q * 32) << 16);
             const int n_tok = min(NT / 2, p.n_tok - tl.tok0 - half);
@@ -570,11 +594,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) i8_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(leader_empty[a]);
+            if (lane == 0) mbar_arrive_remote(leader_empty0 + a * 8);
         }
         __syncwarp();
     }
-    __syncwarp();
+    __syncthreads();
+    if (warp == 1) await_mmas(smem_u32(&drained));
     tc_fence_before();
     cluster_sync();  // the other CTA may still read this one's operands or signal its barriers
     if (warp == 1) {
@@ -597,7 +622,8 @@ int launch_pair(const I8Product& p, int sm_count, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    HB_CUDA(cudaLaunchKernelEx(&cfg, p.accumulate ? i8_pair_kernel<NT, true> : i8_pair_kernel<NT, false>, p, row_pairs, tok_tiles));
+    HB_CUDA(cudaLaunchKernelEx(&cfg, p.accumulate ? i8_pair_kernel<NT, true> : i8_pair_kernel<NT, false>, p, *static_cast<const CUtensorMap*>(p.w_map),
+                               *static_cast<const CUtensorMap*>(NT == 256 ? p.x_map_n256 : p.x_map_n128), row_pairs, tok_tiles));
     return 0;
 }
 
