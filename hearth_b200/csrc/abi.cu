@@ -380,6 +380,7 @@ int current_slot() { return g_cur; }
 cudaStream_t slot_stream() { return g_ctx.stream; }
 int slot_sm_count() { return g_ctx.sm_count; }
 int* slot_status() { return g_ctx.d_status; }
+int take_device_status() { return check_device_status(); }
 }  // namespace hb200
 
 // Binds slot `slot` to CUDA device `device`: stream, status word, scratch, per-device kernel attributes.

@@ -98,6 +98,8 @@ int current_slot();
 cudaStream_t slot_stream();
 int slot_sm_count();
 int* slot_status();
+// After a synchronising call: what the kernels recorded in the status word, as an error code; clears it.
+int take_device_status();
 #define HB_CUDA(expr)                                                                        \
     do {                                                                                     \
         cudaError_t _e = (expr);                                                             \

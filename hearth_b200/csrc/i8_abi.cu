@@ -533,7 +533,7 @@ extern "C" int hb200_matmul_i8(hb200_weight_i8_t w, const float* x, size_t seq_l
     if ((rc = product(w, g.act, seq_len, g.out, w->n_rows, 0, st))) return rc;
     HB_CUDA(cudaMemcpyAsync(out, g.out, out_bytes, cudaMemcpyDeviceToHost, st));
     HB_CUDA(cudaStreamSynchronize(st));
-    return HB200_OK;
+    return take_device_status();  // every product kernel has bounded waits
     I8_END
 }
 
