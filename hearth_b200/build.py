@@ -75,9 +75,10 @@ def _stale(target: str, deps: list[str]) -> bool:
 
 
 # The bounds-checked debug build: the translation units whose kernels carry index checks (and the host layer, which
-# reports them) are compiled again with -DHB200_BOUNDS; the others are shared with the normal build.
+# reports them, and the 8-bit product, whose self-test is there) are compiled again with -DHB200_BOUNDS; the others are
+# shared with the normal build.
 BOUNDS_LIB = os.path.join(HERE, "libhearth_b200_bounds.so")
-BOUNDS_SOURCES = ["abi.cu", "quantize.cu", "producers.cu", "gemv_dp4a.cu", "kquant.cu", "noalloc.cu"]
+BOUNDS_SOURCES = ["abi.cu", "quantize.cu", "producers.cu", "gemv_dp4a.cu", "kquant.cu", "noalloc.cu", "i8_gemm.cu", "i8_abi.cu"]
 
 
 def build_bounds(force: bool = False) -> str:

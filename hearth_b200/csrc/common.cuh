@@ -376,6 +376,9 @@ struct I8Product {
     int accumulate;       // out += result
     int* status;          // device word for an expired wait
     const void *w_map, *x_map_n128, *x_map_n256;  // host: tensor maps of the planes (encode_i8_plane); boxes of 128 rows, of 64 and of 128 tokens
+#ifdef HB200_BOUNDS
+    int report_rank;      // self-test: 1 + the rank of a cluster's CTA that reports a wait that ran out (none did)
+#endif
 };
 int i8_gemm_prepare(int sm_count);  // per device: kernel attributes, clusters that fit at once
 int launch_i8_gemm(const I8Product& p, cudaStream_t st);
@@ -385,5 +388,9 @@ const char* i8_gemm_kernel_name(int n_rows, int kb, int n_tok);
 int encode_i8_plane(void* map, const int8_t* q, size_t rows, size_t blocks, size_t block_stride, int box_rows);
 // i8_abi.cu: frees what the host-buffer product keeps for a slot.
 void i8_release_slot(int slot);
+#ifdef HB200_BOUNDS
+// i8_abi.cu: products one CTA of which reports a failure must store nothing of that CTA's tile.
+int i8_failure_selftest();
+#endif
 
 }  // namespace hb200

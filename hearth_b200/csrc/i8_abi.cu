@@ -5,6 +5,7 @@
 
 #include <cfloat>
 #include <new>
+#include <vector>
 
 #include "../../include/hb200.h"
 #include "common.cuh"
@@ -202,8 +203,11 @@ int check_product(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, size_t 
     return check_ld("ld_out", ld_out, w->n_rows);
 }
 
-int product(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, float* out, size_t ld_out, int accumulate, cudaStream_t st) {
+int product(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, float* out, size_t ld_out, int accumulate, cudaStream_t st, int report_rank = 0) {
     I8Product p = {};
+#ifdef HB200_BOUNDS
+    p.report_rank = report_rank;
+#endif
     p.w = w->plane.q;
     p.sw = w->scales;
     p.a = a->plane.q;
@@ -554,4 +558,43 @@ void i8_release_slot(int slot) {
     }
     g = Staging();
 }
+
+#ifdef HB200_BOUNDS
+int i8_failure_selftest() {
+    // 9 tokens x 2048 columns x 200 rows: two row tiles, each cut over the eight CTAs of a cluster; all operands 1, all scales one float
+    constexpr size_t TOK = 9, COLS = 2048, ROWS = 200;
+    cudaStream_t st = slot_stream();
+    int8_t* q = nullptr;
+    float *s = nullptr, *out = nullptr;
+    hb200_weight_i8_t w = nullptr;
+    hb200_act_i8_t a = nullptr;
+    std::vector<float> got(TOK * ROWS);
+    HB_CUDA(cudaMalloc(&q, ROWS * COLS));
+    HB_CUDA(cudaMalloc(&s, ROWS * sizeof(float)));
+    HB_CUDA(cudaMalloc(&out, got.size() * sizeof(float)));
+    HB_CUDA(cudaMemset(q, 1, ROWS * COLS));
+    HB_CUDA(cudaMemset(s, 0x3F, ROWS * sizeof(float)));
+    HB_CUDA(cudaDeviceSynchronize());
+    int rc = hb200_weight_i8_upload_dev(ROWS, COLS, q, COLS, s, st, &w);
+    if (!rc) rc = hb200_act_i8_create(TOK, COLS, &a);
+    if (!rc) rc = hb200_act_i8_load_dev(a, q, COLS, s, TOK, st);
+    for (int rank = -1; rank < 8 && !rc; rank++) {
+        HB_CUDA(cudaMemsetAsync(out, 0, got.size() * sizeof(float), st));
+        if ((rc = product(w, a, TOK, out, ROWS, 0, st, rank + 1))) break;
+        HB_CUDA(cudaMemcpyAsync(got.data(), out, got.size() * sizeof(float), cudaMemcpyDeviceToHost, st));
+        HB_CUDA(cudaStreamSynchronize(st));
+        const int want = rank < 0 ? HB200_OK : HB200_ERR_TIMEOUT, status = take_device_status();
+        size_t stored = 0;
+        for (float v : got) stored += v != 0.0f;
+        if (status != want || stored != (rank < 0 ? got.size() : 0)) {
+            set_error("8-bit product self-test: rank %d reports a failure, status %d, %zu of %zu outputs stored", rank, status, stored, got.size());
+            rc = HB200_ERR_CUDA;
+        }
+    }
+    if (a) hb200_act_i8_free(a);
+    if (w) hb200_weight_i8_free(w);
+    cudaFree(q); cudaFree(s); cudaFree(out);
+    return rc;
+}
+#endif
 }  // namespace hb200

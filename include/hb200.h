@@ -121,7 +121,9 @@ HB200_API int hb200_bounds_checked(void);
 /* Bounds-checked build only (HB200_ERR_UNSUPPORTED otherwise): runs the
  * quantizer with a block-value pitch that is too small on purpose, over buffers
  * that are large enough, and returns HB200_OK if exactly the stores beyond the
- * pitch were counted and skipped.  Nothing faults. */
+ * pitch were counted and skipped; then 8-bit products one CTA of which reports
+ * a wait that ran out (none does), which must store nothing of that CTA's tile
+ * and give HB200_ERR_TIMEOUT.  Nothing faults. */
 HB200_API int hb200_bounds_selftest(void);
 
 /* The split of a work list over persistent CTAs that hb200_batch_seal uses:

@@ -1,8 +1,13 @@
 """GPU tests of what the 8-bit product reports when a bounded wait on the device has run out."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 import i8_ref as R
+from test_bounds_build import ROOT, bounds_lib
 from test_gpu_peers import _build_rank
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +40,12 @@ def test_the_host_buffer_product_reports_an_expired_wait(hb):
             h.free()
         for b in bufs:
             b.close()
+
+
+def test_a_cta_without_sums_keeps_its_whole_cluster_from_storing():
+    """Of the CTAs that finish a tile together, each in turn reports a wait that ran out (the debug build's self-test: nothing does,
+    and every sum is complete): its neighbours must leave the outputs as they were, too."""
+    code = ("from hearth_b200 import api, lib; api.init(0); l = lib.load(); rc = l.hb200_bounds_selftest(); "
+            "assert rc == 0, (rc, l.hb200_last_error()); assert api.matmul_i8_kernel(200, 2048, 9) == 'i8_tcgen05_n16_split'; print('selftest ok')")
+    p = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env=dict(os.environ, HB200_LIB=bounds_lib()), capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0 and "selftest ok" in p.stdout, (p.stdout + p.stderr)[-2000:]
