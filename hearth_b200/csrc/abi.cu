@@ -377,6 +377,9 @@ namespace hb200 {
 int bound_device() { return g_ctx.ready ? g_ctx.device : -1; }
 int use_slot_of(int slot) { return use_slot(slot); }
 int current_slot() { return g_cur; }
+void restore_slot(int slot) {
+    if (slot != g_cur) g_cur = slot;
+}
 cudaStream_t slot_stream() { return g_ctx.stream; }
 int slot_sm_count() { return g_ctx.sm_count; }
 int* slot_status() { return g_ctx.d_status; }

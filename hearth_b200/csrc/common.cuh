@@ -95,6 +95,8 @@ int bound_device();
 int use_slot_of(int slot);
 // The current slot, and what a call on it needs: the stream of the host-buffer calls, the SM count, the status word.
 int current_slot();
+// Makes `slot` the current one again behind use_slot_of; the thread's device is the caller's to put back with it.
+void restore_slot(int slot);
 cudaStream_t slot_stream();
 int slot_sm_count();
 int* slot_status();

@@ -32,11 +32,12 @@ struct hb200_act_i8 {
 
 namespace {
 
-// The calling thread's device is the slot's inside a call and what it was before afterwards.
+// Inside a call the object's slot is the current one and the calling thread is on its device; afterwards both are what
+// they were (one without the other would have the next object created on a device that is not its slot's).
 struct DeviceScope {
-    int prev = -1;
+    int prev = -1, prev_slot;
     int rc = 0;
-    explicit DeviceScope(int slot) {
+    explicit DeviceScope(int slot) : prev_slot(current_slot()) {
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
         rc = use_slot_of(slot);
         if (rc) return;
@@ -49,6 +50,7 @@ struct DeviceScope {
     }
     ~DeviceScope() {
         if (prev >= 0 && prev != bound_device()) cudaSetDevice(prev);
+        restore_slot(prev_slot);
     }
 };
 

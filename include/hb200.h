@@ -387,7 +387,8 @@ HB200_API int hb200_matmul_f32_noalloc(hb200_weight_t w, const float *x_dev, siz
  * return; they keep no scratch, so calls on different handles may overlap and several products may read one activation
  * at once.  A call that writes an activation must be ordered behind the calls that read it, like any buffer.  seq_len 0
  * is a no-op.  Rows of an activation or an output behind seq_len, and output columns behind n_rows, are left as they
- * were. */
+ * were.  Weights and activations are created in the current slot; a call on them works in theirs and leaves the current
+ * slot, and the thread's current device, as they were. */
 #define HB200_I8_MAX_COLS 65536
 #define HB200_I8_MAX_ROWS 8388480
 /* int8 values [n_rows][n_cols] and n_rows scales, host memory; the copy on the device is re-tiled. */
