@@ -116,6 +116,23 @@ int check_ld(const char* what, size_t ld, size_t least) {
     return 0;
 }
 
+// Device inputs of the calls that take no handle: memory a kernel on the current slot's device can read (nothing else ties
+// them to that device, and reading memory of another one, or of the host, would be a fault).
+int check_memory(const char* what, const void* p) {
+    cudaPointerAttributes at = {};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess || at.type == cudaMemoryTypeUnregistered) {
+        cudaGetLastError();
+        set_error("%s: not device memory", what);
+        return HB200_ERR_BAD_SHAPE;
+    }
+    if (at.type == cudaMemoryTypeDevice && at.device != bound_device()) {
+        set_error("%s: on device %d, the current slot is on device %d", what, at.device, bound_device());
+        return HB200_ERR_BAD_SHAPE;
+    }
+    return 0;
+}
+
 int weight_new(size_t n_rows, size_t n_cols, hb200_weight_i8** out) {
     hb200_weight_i8* w = new hb200_weight_i8();
     w->slot = current_slot();
@@ -269,6 +286,7 @@ extern "C" int hb200_weight_i8_upload_dev(size_t n_rows, size_t n_cols, const in
     if ((rc = check_ld("ld_q", ld_q, n_cols))) return rc;
     if (n_rows > 0 && (!q_dev || !scales_dev)) { set_error("null weight values or scales"); return HB200_ERR_NULL; }
     I8_USE(current_slot());
+    if (n_rows > 0 && ((rc = check_memory("weight values", q_dev)) || (rc = check_memory("weight scales", scales_dev)))) return rc;
     hb200_weight_i8* w = nullptr;
     if ((rc = weight_new(n_rows, n_cols, &w))) return rc;
     rc = launch_i8_load(q_dev, ld_q, scales_dev, (int)n_rows, (int)n_cols, w->plane, w->scales, (cudaStream_t)stream);
@@ -285,6 +303,7 @@ extern "C" int hb200_weight_i8_quantize_dev(size_t n_rows, size_t n_cols, const 
     if ((rc = check_ld("ld_w", ld_w, n_cols))) return rc;
     if (n_rows > 0 && !w_dev) { set_error("null weight values"); return HB200_ERR_NULL; }
     I8_USE(current_slot());
+    if (n_rows > 0 && (rc = check_memory("weight values", w_dev))) return rc;
     hb200_weight_i8* w = nullptr;
     if ((rc = weight_new(n_rows, n_cols, &w))) return rc;
     I8Rows p = {};

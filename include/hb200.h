@@ -398,7 +398,8 @@ HB200_API int hb200_weight_i8_upload(size_t n_rows, size_t n_cols, const int8_t 
 HB200_API int hb200_weight_i8_upload_rows(size_t n_rows, size_t n_cols, const int8_t *q, const float *scales,
                                           size_t row_begin, size_t row_end, hb200_weight_i8_t *out);
 /* The same from device memory, rows ld_q bytes apart, read on `stream`.  This call and the next synchronise `stream`
- * (the weight is complete when they return), so they cannot be captured into a graph. */
+ * (the weight is complete when they return), so they cannot be captured into a graph.  Memory of another device than the
+ * current slot's, or of the host, is refused (HB200_ERR_BAD_SHAPE). */
 HB200_API int hb200_weight_i8_upload_dev(size_t n_rows, size_t n_cols, const int8_t *q_dev, size_t ld_q,
                                          const float *scales_dev, void *stream, hb200_weight_i8_t *out);
 /* Rounds f32 weights [n_rows][n_cols], rows ld_w floats apart in device memory, to 8 bits row by row. */
