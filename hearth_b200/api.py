@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 import numpy as np
 
@@ -459,6 +460,29 @@ _F32 = _I8 = _raw_stream = None  # torch.float32, torch.int8 and the current str
 _fast = None  # the compiled checks and calls (csrc/pycall.cpp): a status code, or None for whatever is not the usual case
 
 
+class _ChecksInPython:
+    """In the place of the compiled calls where they cannot be used: every call is left to the checks below."""
+    quantize = add_rms_norm = silu_mul = dequantize = matmul = staticmethod(lambda *args: None)
+
+
+def _compiled_calls():
+    """The extension module, if it was built from the headers of the interpreter and the torch that run now: its code reads
+    tensors directly, so one of another torch could hand the kernels wrong addresses."""
+    from . import build
+    try:
+        from . import _pycall
+    except ImportError as e:
+        why = str(e)
+    else:
+        made, wanted = getattr(_pycall, "built_for", "another torch"), build.pycall_for()
+        if made == wanted:
+            return _pycall
+        why = f"built for {made}, this is {wanted}"
+    warnings.warn(f"hearth_b200/_pycall.so is not used ({why}): the calls of the 8-bit linear path are checked in Python, a few "
+                  "microseconds each; `python -m hearth_b200.build` makes it")
+    return None
+
+
 def _i8_torch() -> None:
     """Binds the torch names the calls below use, and the compiled calls: at one token a call's checks would otherwise
     cost more than its kernel."""
@@ -466,16 +490,14 @@ def _i8_torch() -> None:
     if _F32 is not None:
         return
     import torch
-    try:
-        from . import _pycall
-    except ImportError as e:
-        raise ImportError("hearth_b200/_pycall.so is missing or was built for another torch: build it with `python -m hearth_b200.build`") from e
     L = _l.load()
     raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
-    hot = ("hb200_act_i8_quantize_dev", "hb200_act_i8_add_rms_norm_dev", "hb200_act_i8_silu_mul_dev", "hb200_act_i8_dequantize_dev",
-           "hb200_matmul_i8_dev")
-    _pycall.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in hot))
-    _F32, _I8, _raw_stream, _fast = torch.float32, torch.int8, raw_stream, _pycall
+    fast = _compiled_calls()
+    if fast is not None:
+        hot = ("hb200_act_i8_quantize_dev", "hb200_act_i8_add_rms_norm_dev", "hb200_act_i8_silu_mul_dev", "hb200_act_i8_dequantize_dev",
+               "hb200_matmul_i8_dev")
+        fast.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in hot))
+    _F32, _I8, _raw_stream, _fast = torch.float32, torch.int8, raw_stream, fast or _ChecksInPython
 
 
 def _i8_rows(name: str, t, dtype, n_cols: int, rows: int, device: int):

@@ -10,6 +10,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -44,26 +45,48 @@ def _headers() -> list[str]:
 PYCALL = os.path.join(HERE, "_pycall.so")
 
 
+def pycall_for() -> str:
+    """The interpreter and the torch whose layouts a build of pycall.cpp reads; the module carries this text as `built_for`."""
+    import torch
+    return f"{sys.implementation.cache_tag} torch {torch.__version__} {torch.version.git_version}"
+
+
+def _pycall_stale(src: str) -> bool:
+    if _stale(PYCALL, [src]):
+        return True
+    with open(PYCALL, "rb") as f:  # (read, not imported: a loaded module could not be replaced)
+        return pycall_for().encode() + b"\0" not in f.read()
+
+
 def build_pycall(force: bool = False) -> str | None:
-    """None where there is no torch with CUDA: the calls it serves take CUDA tensors."""
+    """None where there is no torch with CUDA (the calls it serves take CUDA tensors), or, with a warning, where it cannot be compiled
+    (api.py then makes the same checks in Python)."""
     src = os.path.join(CSRC, "pycall.cpp")
-    if force or _stale(PYCALL, [src]):
-        try:
-            import torch
-        except ImportError:
-            return None
-        root = os.path.dirname(torch.__file__)
-        if not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
-            return None
+    try:
+        import torch
+    except ImportError:
+        return None
+    root = os.path.dirname(torch.__file__)
+    if not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
+        return None
+    if force or _pycall_stale(src):
         cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
         include = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                    os.path.join(cuda, "include")]
-        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-        cmd += [f"-I{d}" for d in include] + [src, "-o", PYCALL, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-        p = subprocess.run(cmd, capture_output=True, text=True)
-        if p.returncode:
-            sys.stderr.write(p.stdout + p.stderr)
-            raise RuntimeError("g++ failed on pycall.cpp")
+        fresh = PYCALL + ".new"
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DHB_BUILT_FOR="{pycall_for()}"']
+        cmd += [f"-I{d}" for d in include] + [src, "-o", fresh, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+        try:
+            p = subprocess.run(cmd, capture_output=True, text=True)
+            failed, said = p.returncode != 0, p.stdout + p.stderr
+        except OSError as e:
+            failed, said = True, f"{e}\n"
+        if failed:
+            sys.stderr.write(said)
+            warnings.warn("pycall.cpp was not compiled: the calls of the 8-bit linear path are checked in Python, a few microseconds each")
+            return None
+        os.replace(fresh, PYCALL)
     return PYCALL
 
 

@@ -209,5 +209,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", "Checked calls of the 8-
 
 PyMODINIT_FUNC PyInit__pycall(void) {
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
-    return s_cuda_stream ? PyModule_Create(&module) : nullptr;
+    PyObject* m = s_cuda_stream ? PyModule_Create(&module) : nullptr;
+    // the interpreter and torch whose headers were read above (build.py); api.py compares
+    if (m && PyModule_AddStringConstant(m, "built_for", HB_BUILT_FOR) != 0) {
+        Py_DECREF(m);
+        m = nullptr;
+    }
+    return m;
 }
