@@ -102,10 +102,13 @@ int slot_sm_count();
 int* slot_status();
 // After a synchronising call: what the kernels recorded in the status word, as an error code; clears it.
 int take_device_status();
+// A failed call's error is returned here and taken out of the runtime's own record: whoever asks that next (torch, behind its
+// own next launch) would take it for its own.
 #define HB_CUDA(expr)                                                                        \
     do {                                                                                     \
         cudaError_t _e = (expr);                                                             \
         if (_e != cudaSuccess) {                                                             \
+            (void)cudaGetLastError();                                                        \
             hb200::set_error("%s failed: %s (%s:%d)", #expr, cudaGetErrorString(_e), __FILE__, __LINE__); \
             return -6; /* HB200_ERR_CUDA */                                                  \
         }                                                                                    \

@@ -36,3 +36,20 @@ def test_memory_of_another_device_is_refused(hb):
         hb.WeightI8.quantize_dev(torch.ones(4, 128, device="cuda:1"))
     with pytest.raises(hb.Hb200Error, match="device 1"):
         hb.WeightI8.upload_dev(torch.ones(4, 128, dtype=torch.int8, device="cuda:1"), torch.ones(4, device="cuda:1"))
+
+
+def test_a_call_that_runs_out_of_memory_leaves_no_error_behind(hb):
+    """The host-buffer product of a size whose output (2.2 TB) no device holds: refused by the allocator, and neither the next launch of
+    torch nor the library's own takes the error for its own."""
+    import torch
+    from hearth_b200 import lib
+    rows, tok = 8388480, 65535
+    W = hb.WeightI8.upload_dev(torch.ones(rows, 1, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda"))
+    x, out = np.ones(tok, dtype=np.float32), np.zeros(1, dtype=np.float32)
+    assert lib.load().hb200_matmul_i8(W._h, x.ctypes.data, tok, out.ctypes.data) == -6  # (before anything is written to `out`)
+    torch.ones(3, device="cuda").add_(1)
+    W.free()
+    W = hb.WeightI8.upload(np.ones((3, 128), dtype=np.int8), np.ones(3, dtype=np.float32))
+    assert lib.load().hb200_matmul_i8(W._h, np.ones(128, dtype=np.float32).ctypes.data, 1, (got := np.zeros(3, dtype=np.float32)).ctypes.data) == 0
+    assert (got == np.float32(np.float32(127 * 128) * (np.float32(1) / np.float32(127)))).all()
+    W.free()
