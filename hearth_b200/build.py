@@ -6,7 +6,9 @@ in parallel and are re-built only when their source or a header is newer.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
+import runpy
 import subprocess
 import sys
 import sysconfig
@@ -46,9 +48,15 @@ PYCALL = os.path.join(HERE, "_pycall.so")
 
 
 def pycall_for() -> str:
-    """The interpreter and the torch whose layouts a build of pycall.cpp reads; the module carries this text as `built_for`."""
-    import torch
-    return f"{sys.implementation.cache_tag} torch {torch.__version__} {torch.version.git_version}"
+    """The interpreter and the torch whose layouts a build of pycall.cpp reads; the module carries this text as `built_for`.  (torch
+    is not imported for it.)"""
+    version = runpy.run_path(os.path.join(_torch_root(), "version.py"))
+    return f"{sys.implementation.cache_tag} torch {version['__version__']} {version['git_version']}"
+
+
+def _torch_root() -> str | None:
+    spec = importlib.util.find_spec("torch")
+    return os.path.dirname(spec.origin) if spec and spec.origin else None
 
 
 def _pycall_stale(src: str) -> bool:
@@ -62,14 +70,11 @@ def build_pycall(force: bool = False) -> str | None:
     """None where there is no torch with CUDA (the calls it serves take CUDA tensors), or, with a warning, where it cannot be compiled
     (api.py then makes the same checks in Python)."""
     src = os.path.join(CSRC, "pycall.cpp")
-    try:
-        import torch
-    except ImportError:
-        return None
-    root = os.path.dirname(torch.__file__)
-    if not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
+    root = _torch_root()
+    if root is None or not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
         return None
     if force or _pycall_stale(src):
+        import torch
         cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
         include = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                    os.path.join(cuda, "include")]
