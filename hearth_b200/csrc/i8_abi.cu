@@ -68,6 +68,10 @@ struct DeviceScope {
 #define I8_USE(slot)              \
     DeviceScope _scope(slot);     \
     if (_scope.rc) return _scope.rc
+// For a call whose kernels read an object: the object outlives hb200_shutdown, and its slot may be bound to another device since.
+#define I8_USE_OF(obj)            \
+    I8_USE((obj)->slot);          \
+    if (const int _rc = check_device((obj)->device)) return _rc
 
 // Host-buffer product: staging kept per slot and grown on demand.
 struct Staging {
@@ -84,6 +88,12 @@ int need_init() {
         return HB200_ERR_NOT_INITIALIZED;
     }
     return 0;
+}
+
+int check_device(int device) {
+    if (device == bound_device()) return 0;
+    set_error("the object lives on device %d, its slot is bound to device %d now", device, bound_device());
+    return HB200_ERR_NOT_INITIALIZED;
 }
 
 int grow_floats(float** p, size_t* have, size_t want) {
@@ -216,6 +226,7 @@ I8Rows rows_of(hb200_act_i8_t a) {
 int check_product(hb200_weight_i8_t w, hb200_act_i8_t a, size_t seq_len, size_t ld_out) {
     if (!w || !a) { set_error("null weight or activation handle"); return HB200_ERR_NULL; }
     if (a->slot != w->slot) { set_error("the weight lives in device slot %d, the activation in slot %d", w->slot, a->slot); return HB200_ERR_BAD_SHAPE; }
+    if (a->device != w->device) { set_error("the weight lives on device %d, the activation on device %d", w->device, a->device); return HB200_ERR_BAD_SHAPE; }
     if (a->n_cols != w->n_cols) { set_error("dim mismatch: weight has %zu columns, activation %zu", w->n_cols, a->n_cols); return HB200_ERR_BAD_SHAPE; }
     int rc = check_seq(a, seq_len);
     if (rc) return rc;
@@ -323,7 +334,7 @@ extern "C" int hb200_weight_i8_store_dev(hb200_weight_i8_t w, int8_t* q_dev, siz
     if (rc) return rc;
     if (!w) { set_error("null weight handle"); return HB200_ERR_NULL; }
     if (q_dev && (rc = check_ld("ld_q", ld_q, w->n_cols))) return rc;
-    I8_USE(w->slot);
+    I8_USE_OF(w);
     return launch_i8_store(w->plane, w->scales, (int)w->n_rows, (int)w->n_cols, q_dev, ld_q, scales_dev, (cudaStream_t)stream);
     I8_END
 }
@@ -418,7 +429,7 @@ extern "C" int hb200_act_i8_quantize_dev(hb200_act_i8_t a, const float* x_dev, s
     if ((rc = check_ld("ld_x", ld_x, a->n_cols))) return rc;
     if (seq_len == 0) return HB200_OK;
     if (!x_dev) { set_error("null pointer"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     I8Rows p = rows_of(a);
     p.x = x_dev;
     p.ld = ld_x;
@@ -442,7 +453,7 @@ extern "C" int hb200_act_i8_add_rms_norm_dev(hb200_act_i8_t a, const float* x_de
     }
     if (seq_len == 0) return HB200_OK;
     if (!x_dev || !weight_dev) { set_error("null pointer"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     I8Rows p = rows_of(a);
     p.x = x_dev;
     p.y = residual_dev;
@@ -464,7 +475,7 @@ extern "C" int hb200_act_i8_silu_mul_dev(hb200_act_i8_t a, const float* gate_dev
     if ((rc = check_ld("ld", ld, a->n_cols))) return rc;
     if (seq_len == 0) return HB200_OK;
     if (!gate_dev || !up_dev) { set_error("null pointer"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     I8Rows p = rows_of(a);
     p.x = gate_dev;
     p.y = up_dev;
@@ -482,7 +493,7 @@ extern "C" int hb200_act_i8_load_dev(hb200_act_i8_t a, const int8_t* q_dev, size
     if ((rc = check_ld("ld_q", ld_q, a->n_cols))) return rc;
     if (seq_len == 0) return HB200_OK;
     if (!q_dev || !scales_dev) { set_error("null pointer"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     return launch_i8_load(q_dev, ld_q, scales_dev, (int)seq_len, (int)a->n_cols, a->plane, a->scales, (cudaStream_t)stream);
     I8_END
 }
@@ -496,7 +507,7 @@ extern "C" int hb200_act_i8_store_dev(hb200_act_i8_t a, int8_t* q_dev, size_t ld
     if (q_dev && (rc = check_ld("ld_q", ld_q, a->n_cols))) return rc;
     if (seq_len == 0) return HB200_OK;
     if (!q_dev && !scales_dev) { set_error("nothing to store into"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     return launch_i8_store(a->plane, a->scales, (int)seq_len, (int)a->n_cols, q_dev, ld_q, scales_dev, (cudaStream_t)stream);
     I8_END
 }
@@ -510,7 +521,7 @@ extern "C" int hb200_act_i8_dequantize_dev(hb200_act_i8_t a, float* out_dev, siz
     if ((rc = check_ld("ld_out", ld_out, a->n_cols))) return rc;
     if (seq_len == 0) return HB200_OK;
     if (!out_dev) { set_error("null output"); return HB200_ERR_NULL; }
-    I8_USE(a->slot);
+    I8_USE_OF(a);
     return launch_i8_dequantize(a->plane, a->scales, (int)seq_len, (int)a->n_cols, out_dev, ld_out, (cudaStream_t)stream);
     I8_END
 }
@@ -525,7 +536,7 @@ extern "C" int hb200_matmul_i8_dev(hb200_weight_i8_t w, hb200_act_i8_t a, size_t
     if ((rc = check_product(w, a, seq_len, ld_out))) return rc;
     if (seq_len == 0 || w->n_rows == 0) return HB200_OK;
     if (!out_dev) { set_error("null output"); return HB200_ERR_NULL; }
-    I8_USE(w->slot);
+    I8_USE_OF(w);
     return product(w, a, seq_len, out_dev, ld_out, accumulate, (cudaStream_t)stream);
     I8_END
 }
@@ -538,7 +549,7 @@ extern "C" int hb200_matmul_i8(hb200_weight_i8_t w, const float* x, size_t seq_l
     if (seq_len > HB200_MAX_SEQ_LEN) { set_error("seq_len %zu (limit %d)", seq_len, HB200_MAX_SEQ_LEN); return HB200_ERR_TOO_LARGE; }
     if (seq_len == 0 || w->n_rows == 0) return HB200_OK;
     if (!x || !out) { set_error("null buffer"); return HB200_ERR_NULL; }
-    I8_USE(w->slot);
+    I8_USE_OF(w);
     Staging& g = g_staging[w->slot];
     const size_t in_bytes = seq_len * w->n_cols * sizeof(float), out_bytes = seq_len * w->n_rows * sizeof(float);
     if ((rc = grow_floats(&g.x, &g.x_bytes, in_bytes))) return rc;

@@ -53,3 +53,27 @@ def test_a_call_that_runs_out_of_memory_leaves_no_error_behind(hb):
     assert lib.load().hb200_matmul_i8(W._h, np.ones(128, dtype=np.float32).ctypes.data, 1, (got := np.zeros(3, dtype=np.float32)).ctypes.data) == 0
     assert (got == np.float32(np.float32(127 * 128) * (np.float32(1) / np.float32(127)))).all()
     W.free()
+
+
+def test_objects_of_a_slot_that_moved_to_another_device_are_refused(hb):
+    """An object outlives hb200_shutdown; its slot may then be bound to another device.  Here the object's own record of its device (the
+    second int behind the handle) is changed instead: every call that would read it there is refused, freeing is not."""
+    import torch
+    W, A, B = hb.WeightI8.quantize_dev(torch.ones(4, 128, device="cuda")), hb.ActI8(2, 128), hb.ActI8(2, 128)
+    x, q, s = torch.ones(2, 128, device="cuda"), torch.ones(4, 128, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    w, out = torch.ones(128, device="cuda"), torch.full((2, 4), 5.0, device="cuda")
+    B.quantize(x, 2)
+    for h in (W, A):
+        record = C.c_int.from_address(h._p + 4)
+        assert record.value == h.device
+        record.value = h.device + 1
+    calls = [lambda: A.quantize(x, 2), lambda: A.add_rms_norm(x, w, 1e-6, 2), lambda: A.silu_mul(x, x, 2), lambda: A.load(q, s, 2), lambda: A.store(q, s, 2),
+             lambda: A.dequantize(x, 2), lambda: W.store(q, s), lambda: hb.matmul_i8_dev(W, A, 2, out), lambda: hb.matmul_i8_dev(W, B, 2, out),
+             lambda: hb.matmul_i8(W, np.ones((2, 128), dtype=np.float32))]
+    for i, call in enumerate(calls):
+        with pytest.raises(hb.Hb200Error, match="device"):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    assert (out == 5).all()
+    for h in (W, A, B):
+        h.free()
