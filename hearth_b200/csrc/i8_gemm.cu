@@ -19,10 +19,11 @@
 //
 // Measured (back to back in a graph, us; weight bytes per second or operations per second):
 //   1 x 2048 x 151669   47.0 (6.6 TB/s, the copy bandwidth)      4 x 5120 x 34816    27.5 (6.5 TB/s)
-//   1 x 4096 x 4096      4.2 (weights in L2)                     16 x 4096 x 24576   18.0 (5.6 TB/s)
-//   32 x 17408 x 5120   16.3 (5.5 TB/s)                          77 x 12288 x 4096   14.5 (3.5 TB/s)
-//   512 x 4096 x 24576  44.5 (2 320 TOP/s)                       4096 x 5120 x 17408  234 (3 120 TOP/s; 94 % of the tensor
-// pipe's cycles; after a second of it the GPU is at its 1000 W limit and 1.35 GHz, and it takes 270).
+//   1 x 4096 x 4096      4.3 (weights in L2)                     16 x 4096 x 24576   17.7 (5.7 TB/s)
+//   32 x 17408 x 5120   16.4 (5.4 TB/s)                          77 x 12288 x 4096   14.5 (3.5 TB/s)
+//   512 x 4096 x 24576  44.2 (2 330 TOP/s)                       4096 x 5120 x 17408  236 (3 090 TOP/s)
+// The last two before the GPU throttles.  After two seconds of the last it takes 273 (2 680 TOP/s) at the 1000 W limit and a sampled
+// median of 1.37 GHz: 373 000 cycles, of which its MMAs are 307 000 (15 rounds of tiles x 20 stages x 1 024).
 // Between 33 and 128 tokens a third of the time is not streaming: from a kernel's end to its successor's wait 2 us, the
 // exchange of the partial sums 2 us (a CTA stores about 8 bytes a clock into its neighbours), barrier and output 2 us.
 //

@@ -8,8 +8,9 @@
 //
 // The norm's factor multiplies every value of its row, so it cancels out of q and only the scale carries it: one pass
 // over the row computes h, the maximum and the sum of squares together, and the int8 values do not depend on the order
-// of that sum.  All steps are f32 with IEEE rounding (h, v, 127 / a and the product each rounded once), so q is
-// determined to the last bit; never compile this file with fast-math.  A row whose maximum is below I8_MIN_MAX (2^-100,
+// of that sum.  All steps are f32 with IEEE rounding (h, v, 127 / a and the product each rounded once), so for quantize and
+// the norm q is determined to the last bit; silu_mul's v is within five half units of the exact value, since expf is within
+// one unit.  Never compile this file with fast-math.  A row whose maximum is below I8_MIN_MAX (2^-100,
 // where 127 / a would leave the range of f32) is stored as zeros with scale 0.  A row with an infinity or a NaN in it (or
 // whose sum of squares overflows) is stored as zeros with scale NaN, so whatever is computed from it is NaN, too.
 //
@@ -17,7 +18,7 @@
 // row (a cluster of eight for a few long rows) keeps the row in registers between the reduction and the rounding, up to
 // 32 values a thread; many rows of more than 32768 columns are read twice.  Measured: quantize of 4096 x 4096 13.7 us
 // (6.1 TB/s), add_rms_norm 36 us (6.1 TB/s), silu_mul 26 us (5.8 TB/s), of 512 x 17408 19.5 us (4.1 TB/s: two rows are all
-// that fit an SM's registers, and they load and compute in step), one row of 4096 columns 1.5 / 2.3 / 1.9 us behind its
+// that fit an SM's registers, and they load and compute in step; 56 registers with 36 bytes of spills a thread), one row of 4096 columns 1.5 / 2.3 / 1.9 us behind its
 // predecessor in a graph.
 //
 // Reference counterparts with a scale per 32 columns: ops::rms_norm_q8 and ops::silu_mul_q8

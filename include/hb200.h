@@ -377,15 +377,16 @@ HB200_API int hb200_matmul_f32_noalloc(hb200_weight_t w, const float *x_dev, siz
  * (hearth-quant/src/q8_0.rs:20-51, hearth-llm/src/ops.rs:273-306, :442-504, hearth-llm/src/model/matmul.rs:580-674).
  *
  * Rounding a row v to 8 bits: a = max |v|, q = v * (127 / a) rounded to the nearest integer (ties to even), scale = a /
- * 127; every step is one f32 operation rounded to nearest, so the integers are determined to the last one.  A row with
+ * 127; every step is one f32 operation rounded to nearest, so the integers of a given v are determined to the last one (v
+ * itself too, but for the gated activation: its exp is within a unit in the last place).  A row with
  * a < 2^-100 becomes zeros with scale 0.  A row holding an infinity or a NaN becomes zeros with scale NaN: every output
  * of that token is NaN, and no other token's.  Values handed in by the caller may use all of -128 .. 127.
  *
  * Limits: n_cols <= HB200_I8_MAX_COLS, n_rows <= HB200_I8_MAX_ROWS, HB200_MAX_SEQ_LEN tokens; beyond them
  * HB200_ERR_TOO_LARGE.  Rows of f32 inputs and outputs are `ld` floats apart (ld >= the row's length, any alignment;
  * multiples of four and 16-byte-aligned bases are faster).  _dev calls enqueue on `stream` (of the handle's device) and
- * return; they keep no scratch, so calls on different handles may overlap and several products may read one activation
- * at once.  A call that writes an activation must be ordered behind the calls that read it, like any buffer.  seq_len 0
+ * return; they keep no scratch, so on the device calls on different handles may overlap and several products may read
+ * one activation at once (the host calls of a context are serialised like all others).  A call that writes an activation must be ordered behind the calls that read it, like any buffer.  seq_len 0
  * is a no-op.  Rows of an activation or an output behind seq_len, and output columns behind n_rows, are left as they
  * were.  Weights and activations are created in the current slot; a call on them works in theirs and leaves the current
  * slot, and the thread's current device, as they were. */
